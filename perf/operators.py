@@ -1,0 +1,352 @@
+"""The measured cases of three operators that serve a batch through the host network on stored features:
+
+  kv_write, kv_read   the key/value cache held in 8 bits: quantised as it is written, read back as numbers
+  shared_attn         attention of a batch whose sequences share a long prefix of keys and values
+  gn_fwd, gn_train    group normalisation with an activation, channels last (forward; forward and backward)
+
+Where `own` is false a pass runs the plain form (elementary torch operations in 32 bits), where it is true the
+package's own operators.
+"""
+import math
+
+import torch
+
+own = False
+
+DEV = "cuda"
+_T = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+_TOP = {"int8": 127.0, "e4m3": 448.0}       # the largest code of each 8-bit format
+_TINY = 2.0 ** -100                         # rows whose largest magnitude is below this are stored as zeros
+
+
+# ------------------------------------------------------------------------------------------------ cases
+
+def listed():
+    return [
+        # one decoding step of 16 sequences appends one token each to its cache
+        dict(name="kv_write one token", op="kv_write", fmt="int8", dtype="bf16", B=16, n=1, H=8, d=64, S=512),
+        # the producer stores one (timestep, layer) entry of four images: fp32 features, 64 x 64 latent
+        dict(name="kv_write entry", op="kv_write", fmt="e4m3", dtype="f32", B=4, n=4096, H=8, d=40, S=4096),
+        # a text context's 77 keys and values, read back for one call
+        dict(name="kv_read context", op="kv_read", fmt="e4m3", dtype="bf16", B=1, n=77, H=8, d=40, S=80),
+        # a layer's entries of eight images read back for a kernel that takes 16-bit tensors, an odd length
+        dict(name="kv_read entry", op="kv_read", fmt="int8", dtype="f16", B=8, n=4001, H=8, d=80, S=4096),
+        # decoding, few sequences: latency counts
+        dict(name="attn decode few", op="shared_attn", dtype="f16", fmt="none", B=4, Hq=8, Hkv=8, n=1, P=1023, S=128, d=64, causal=False),
+        # decoding, 32 sequences with grouped heads behind one long prefix, ragged lengths
+        dict(name="attn decode long", op="shared_attn", dtype="bf16", fmt="none", B=32, Hq=32, Hkv=8, n=1, P=32768, S=1024, d=128, causal=False),
+        # five drafted tokens each, prefix and own keys in the 8-bit cache
+        dict(name="attn draft int8", op="shared_attn", dtype="bf16", fmt="int8", B=16, Hq=16, Hkv=4, n=5, P=8191, S=333, d=128, causal=True),
+        # four images attend to one stored style entry and to their own tokens, 64 x 64 latent
+        dict(name="attn images", op="shared_attn", dtype="bf16", fmt="none", B=4, Hq=8, Hkv=8, n=4096, P=4096, S=4096, d=40, causal=False),
+        # the innermost level of the host network at one image
+        dict(name="gn_fwd 8x8x1280", op="gn_fwd", dtype="f32", B=1, h=8, w=8, C=1280, G=32, act="silu"),
+        # its outermost level with sixteen images
+        dict(name="gn_fwd 64x64x320", op="gn_fwd", dtype="bf16", B=16, h=64, w=64, C=320, G=32, act="silu"),
+        # training: a middle level with two images
+        dict(name="gn_train 16x16x640", op="gn_train", dtype="bf16", B=2, h=16, w=16, C=640, G=32, act="silu"),
+        # training: the widest input of the outermost level (skip connection joined), eight images
+        dict(name="gn_train 64x64x960", op="gn_train", dtype="bf16", B=8, h=64, w=64, C=960, G=32, act="silu"),
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["kv_write", "kv_read", "shared_attn", "shared_attn", "gn_fwd", "gn_train"])
+    if op in ("kv_write", "kv_read"):
+        while True:
+            c = dict(op=op, fmt=rng.choice(["int8", "e4m3"]), dtype=rng.choice(["f32", "bf16", "f16"]), B=_log(rng, 1, 32),
+                     n=_log(rng, 1, 8192), H=rng.randint(1, 16), d=8 * rng.randint(1, 32))
+            c["S"] = c["n"] + rng.choice([0, 1, rng.randint(0, 100)])
+            if c["B"] * c["n"] * c["H"] * c["d"] <= (5 << 20 if op == "kv_write" else 20 << 20):
+                return c
+    if op == "shared_attn":
+        while True:
+            Hkv, group = rng.choice([1, 2, 4, 8]), rng.choice([1, 1, 2, 4, 7, 8])
+            c = dict(op=op, dtype=rng.choice(["bf16", "f16"]), fmt=rng.choice(["none", "none", "int8", "e4m3"]), B=_log(rng, 1, 48),
+                     Hq=Hkv * group, Hkv=Hkv, n=rng.choice([1, rng.randint(2, 9), _log(rng, 1, 4096)]), P=rng.choice([0, _log(rng, 1, 32768), _log(rng, 64, 32768)]),
+                     S=_log(rng, 1, 4096), d=rng.choice([40, 64, 80, 128, 160, 8 * rng.randint(1, 32)]), causal=rng.random() < 0.4)
+            keys = c["P"] + c["S"]
+            if c["B"] * c["Hq"] * c["n"] * keys <= 1 << 29 and c["B"] * c["Hkv"] * c["S"] * c["d"] + c["Hkv"] * c["P"] * c["d"] <= 64 << 20:
+                return c
+    while True:
+        G = rng.choice([1, 2, 8, 16, 32])
+        c = dict(op=op, dtype=rng.choice(["f32", "bf16", "f16"]), B=_log(rng, 1, 16), h=_log(rng, 1, 96), w=_log(rng, 1, 96),
+                 C=G * rng.randint(1, 60), G=G, act=rng.choice(["silu", "silu", "none"]))
+        if c["B"] * c["h"] * c["w"] * c["C"] <= 10 << 20 and c["h"] * c["w"] * c["C"] // G >= 16:
+            return c
+
+
+# ----------------------------------------------------------------------------------------------- inputs
+
+def _lengths(c):
+    """How many of its own keys each sequence of the batch has: from none to all, a matter of the case alone."""
+    B, S = c["B"], c["S"]
+    return [S if b == 0 else 0 if b == 5 else S - (b * 7919 % (S // 2 + 1)) for b in range(B)]
+
+
+def _normal(shape, g, scale=1.0, dtype=torch.float32):
+    return (torch.randn(shape, generator=g, device=DEV) * scale).to(dtype)
+
+
+def _cache(B, H, S, d, fmt, g):
+    """A filled 8-bit cache: codes (B, H, S, d) and one scale per row, of key and value rows of uneven size."""
+    out = {}
+    for x in "kv":
+        rows = _normal((B, H, S, d), g) * torch.exp(0.5 * torch.randn((B, H, S, 1), generator=g, device=DEV))
+        out[x + "_codes"], out[x + "_scale"] = _quantise(rows, fmt)
+    return out
+
+
+def prepare(case, seed):
+    c, g = dict(case), torch.Generator(device=DEV).manual_seed(seed)
+    st = {"case": c}
+    if c["op"] in ("kv_write", "kv_read"):
+        B, n, H, d, S = (c[k] for k in ("B", "n", "H", "d", "S"))
+        st["cache"] = _cache(B, H, S, d, c["fmt"], g)
+        st["start"] = torch.tensor([b * 31 % (S - n + 1) for b in range(B)], dtype=torch.int32, device=DEV)
+        if c["op"] == "kv_write":
+            for x in "kv":      # as a projection leaves them: (B, n, H * d)
+                st[x] = _normal((B, n, H, d), g, dtype=_T[c["dtype"]]).transpose(1, 2)
+    elif c["op"] == "shared_attn":
+        B, Hq, Hkv, n, P, S, d = (c[k] for k in ("B", "Hq", "Hkv", "n", "P", "S", "d"))
+        t = _T[c["dtype"]]
+        st["q"] = _normal((B, n, Hq, d), g, 1.5, t).transpose(1, 2)
+        if c["fmt"] == "none":
+            st["prefix"] = {x: _normal((Hkv, P, d), g, dtype=t) for x in "kv"}
+            st["own"] = {x: _normal((B, Hkv, S, d), g, dtype=t) for x in "kv"}
+        else:
+            st["prefix"] = _cache(1, Hkv, P, d, c["fmt"], g)
+            st["own"] = _cache(B, Hkv, S, d, c["fmt"], g)
+        st["own_len"] = torch.tensor(_lengths(c), dtype=torch.int32, device=DEV)
+    else:
+        B, h, w, C, t = c["B"], c["h"], c["w"], c["C"], _T[c["dtype"]]
+        x = _normal((B, h, w, C), g, 1.3) + 0.5 * torch.randn((C,), generator=g, device=DEV)
+        st["x"] = x.to(t).permute(0, 3, 1, 2)               # (B, C, h, w), channels last in memory
+        st["weight"] = 1.0 + _normal((C,), g, 0.2)
+        st["bias"] = _normal((C,), g, 0.2)
+        if c["op"] == "gn_train":
+            st["dy"] = _normal((B, h, w, C), g, dtype=t).permute(0, 3, 1, 2)
+            for k in ("x", "weight", "bias"):
+                st[k].requires_grad_(True)
+    return st
+
+
+# ------------------------------------------------------------------------------------------- plain forms
+
+def _quantise(rows, fmt):
+    """One scale per row (last axis): codes = round(row * top / max|row|), scale = max|row| / top."""
+    x = rows.float()
+    top = _TOP[fmt]
+    amax = x.abs().amax(-1, keepdim=True)
+    live = amax >= _TINY
+    inv = torch.where(live, top / torch.where(live, amax, 1.0), 0.0)
+    y = (x * inv).clamp(-top, top)
+    codes = torch.round(y).to(torch.int8) if fmt == "int8" else y.to(torch.float8_e4m3fn)
+    return codes, torch.where(live, amax / top, 0.0).squeeze(-1)
+
+
+def _plain_write(st):
+    c, cache = st["case"], st["cache"]
+    B, n = c["B"], c["n"]
+    at = st["start"].long()[:, None] + torch.arange(n, device=DEV)
+    b = torch.arange(B, device=DEV)[:, None].expand(B, n)
+    for x in "kv":
+        codes, scale = _quantise(st[x], c["fmt"])
+        cache[x + "_codes"].view(torch.uint8)[b, :, at] = codes.view(torch.uint8).transpose(1, 2)
+        cache[x + "_scale"][b, :, at] = scale.transpose(1, 2)
+    return cache
+
+
+def _plain_read(st):
+    c, cache = st["case"], st["cache"]
+    B, n = c["B"], c["n"]
+    at = st["start"].long()[:, None] + torch.arange(n, device=DEV)
+    b = torch.arange(B, device=DEV)[:, None].expand(B, n)
+    out = []
+    for x in "kv":
+        codes = cache[x + "_codes"].view(torch.uint8)[b, :, at].view(cache[x + "_codes"].dtype)      # (B, n, H, d)
+        y = codes.float() * cache[x + "_scale"][b, :, at][..., None]
+        out.append(y.transpose(1, 2).contiguous().to(_T[c["dtype"]]))
+    return out
+
+
+def _numbers(src, x):
+    """Keys ("k") or values ("v") of a prefix or of the sequences' own part, in 32 bits."""
+    if x in src:
+        return src[x].float()
+    return src[x + "_codes"].float() * src[x + "_scale"][..., None]
+
+
+def _plain_attn(st):
+    c = st["case"]
+    B, Hq, Hkv, n, P, S, d = (c[k] for k in ("B", "Hq", "Hkv", "n", "P", "S", "d"))
+    G = Hq // Hkv
+    q = st["q"].float().reshape(B, Hkv, G * n, d) * d ** -0.5
+    kp, vp = (_numbers(st["prefix"], x).reshape(Hkv, P, d) for x in "kv")
+    ko, vo = (_numbers(st["own"], x) for x in "kv")
+    lp = torch.matmul(q, kp.transpose(1, 2)).reshape(B, Hq, n, P)
+    lo = torch.matmul(q, ko.transpose(2, 3)).reshape(B, Hq, n, S)
+    row = torch.arange(n, device=DEV)
+    limit = st["own_len"][:, None] + (row - n + 1 if c["causal"] else 0 * row)       # own keys that a row sees: j < limit
+    seen = torch.arange(S, device=DEV) < limit[:, None, :, None]
+    lo = torch.where(seen, lo, -math.inf)
+    m = lo.amax(-1, keepdim=True)
+    if P:
+        m = torch.maximum(m, lp.amax(-1, keepdim=True))
+    m = torch.where(m == -math.inf, 0.0, m)
+    ep, eo = torch.exp(lp - m), torch.exp(lo - m)
+    total = ep.sum(-1, keepdim=True) + eo.sum(-1, keepdim=True)
+    out = torch.matmul(ep.reshape(B, Hkv, G * n, P), vp) + torch.matmul(eo.reshape(B, Hkv, G * n, S), vo)
+    out = out.reshape(B, Hq, n, d) / torch.where(total == 0, 1.0, total)              # a row that sees no key gives zeros
+    return out.transpose(1, 2).reshape(B, n, Hq * d).to(_T[c["dtype"]])
+
+
+def _plain_norm(st):
+    c = st["case"]
+    B, h, w, C, G = (c[k] for k in ("B", "h", "w", "C", "G"))
+    x = st["x"].detach().permute(0, 2, 3, 1).reshape(B, h * w, G, C // G).float()
+    wt, bs = (st[k].detach().float().reshape(G, C // G) for k in ("weight", "bias"))
+    mean = x.mean((1, 3), keepdim=True)
+    rstd = torch.rsqrt((x - mean).square().mean((1, 3), keepdim=True) + 1e-5)
+    xh = (x - mean) * rstd
+    z = xh * wt + bs
+    sig = 1 / (1 + torch.exp(-z))
+    y = (z * sig if c["act"] == "silu" else z).reshape(B, h, w, C).permute(0, 3, 1, 2).to(_T[c["dtype"]])
+    if c["op"] == "gn_fwd":
+        return y
+    dz = st["dy"].permute(0, 2, 3, 1).reshape(B, h * w, G, C // G).float()
+    if c["act"] == "silu":
+        dz = dz * (sig * (1 + z * (1 - sig)))
+    dw, db = (dz * xh).sum((0, 1)).reshape(C), dz.sum((0, 1)).reshape(C)
+    dxh = dz * wt
+    dx = rstd * (dxh - dxh.mean((1, 3), keepdim=True) - xh * (dxh * xh).mean((1, 3), keepdim=True))
+    return y, dx.reshape(B, h, w, C).permute(0, 3, 1, 2).to(_T[c["dtype"]]), dw, db
+
+
+_PLAIN = {"kv_write": _plain_write, "kv_read": _plain_read, "shared_attn": _plain_attn, "gn_fwd": _plain_norm, "gn_train": _plain_norm}
+
+
+# --------------------------------------------------------------------------------- the package's operators
+
+def _own(st):
+    from style_transfer_amd import ops
+    c = st["case"]
+    if c["op"] == "kv_write":
+        ops.kv_cache_write(ops.QuantKV(**st["cache"]), st["k"], st["v"], st["start"])
+        return st["cache"]
+    if c["op"] == "kv_read":
+        return list(ops.kv_cache_read(ops.QuantKV(**st["cache"]), st["start"], c["n"], _T[c["dtype"]]))
+    if c["op"] == "shared_attn":
+        side = [(s["k"], s["v"]) if "k" in s else ops.QuantKV(**s) for s in (st["prefix"], st["own"])]
+        return ops.shared_prefix_attention(st["q"], side[0], side[1], own_len=st["own_len"], causal=c["causal"])
+    y = ops.group_norm_act(st["x"], c["G"], st["weight"], st["bias"], eps=1e-5, act=c["act"])
+    if c["op"] == "gn_fwd":
+        return y
+    return (y.detach(),) + torch.autograd.grad(y, (st["x"], st["weight"], st["bias"]), st["dy"])
+
+
+def run(state):
+    return _own(state) if own else _PLAIN[state["case"]["op"]](state)
+
+
+# -------------------------------------------------------------------------------------------------- work
+
+def work(case):
+    c = case
+    es = 4 if c.get("dtype") == "f32" else 2
+    if c["op"] in ("kv_write", "kv_read"):
+        rows = 2 * c["B"] * c["n"] * c["H"]
+        return {"bytes": rows * (c["d"] * (es + 1) + 4), "flops": 2 * rows * c["d"]}
+    if c["op"] == "shared_attn":
+        B, Hq, Hkv, n, P, d = (c[k] for k in ("B", "Hq", "Hkv", "n", "P", "d"))
+        row = 2 * (d * es if c["fmt"] == "none" else d + 4)                     # a key and its value
+        lens = _lengths(c)
+        pairs = 0
+        for L in lens:
+            pairs += n * P
+            # causal: row i sees min(L, L - n + 1 + i) own keys, not below none
+            pairs += sum(max(0, L - n + 1 + i) for i in range(n)) if c["causal"] else n * L
+        return {"bytes": 2 * B * Hq * n * d * es + Hkv * (P + sum(lens)) * row, "flops": 4 * Hq * d * pairs}
+    els = c["B"] * c["h"] * c["w"] * c["C"]
+    if c["op"] == "gn_fwd":
+        return {"bytes": 2 * els * es + 8 * c["C"], "flops": 12 * els}
+    return {"bytes": 4 * els * es + 16 * c["C"], "flops": 40 * els}             # x, dy read; y, dx written
+
+
+# -------------------------------------------------------------------------------------------- 64-bit values
+
+def _exact_codes(x, fmt):
+    """Codes and scales of rows in 64 bits, by the definition: the code nearest to row / scale."""
+    top = 127.0 if fmt == "int8" else 448.0
+    peak = x.double().abs().max(-1).values
+    scale = peak / top
+    scale[peak < 2.0 ** -100] = 0
+    z = x.double() / torch.where(scale == 0, torch.ones_like(scale), scale)[..., None]
+    if fmt == "int8":
+        return None, scale
+    # e4m3: 3 fraction bits, smallest exponent -6: spacing 2^(e-3)
+    e = torch.floor(torch.log2(z.abs().clamp_min(2.0 ** -6))).clamp(-6, 8)
+    step = torch.exp2(e - 3)
+    return (torch.round(z / step) * step).clamp(-448, 448), scale
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    c = st["case"]
+    if c["op"] in ("kv_write", "kv_read"):
+        n, cache, out = c["n"], st["cache"], {}
+        starts = [b * 31 % (c["S"] - n + 1) for b in range(c["B"])]
+        if c["op"] == "kv_read":
+            res = []
+            for x in "kv":
+                y = cache[x + "_codes"].double() * cache[x + "_scale"].double().unsqueeze(-1)
+                res.append(torch.stack([y[b, :, s:s + n] for b, s in enumerate(starts)]))
+            return res
+        for x in "kv":
+            codes, scale = cache[x + "_codes"].double(), cache[x + "_scale"].double()
+            new, ns = _exact_codes(st[x], c["fmt"])
+            for b, s in enumerate(starts):
+                scale[b, :, s:s + n] = ns[b]
+                if new is not None:
+                    codes[b, :, s:s + n] = new[b]
+            out[x + "_codes"], out[x + "_scale"] = codes if new is not None else None, scale
+        return out
+    if c["op"] == "shared_attn":
+        B, Hq, Hkv, n, P, S, d = (c[k] for k in ("B", "Hq", "Hkv", "n", "P", "S", "d"))
+        res = torch.zeros((B, n, Hq, d), dtype=torch.float64, device=DEV)
+
+        def head(src, x, b, h):
+            if x in src:
+                return src[x][h].double() if b is None else src[x][b, h].double()
+            b = 0 if b is None else b
+            return src[x + "_codes"][b, h].double() * src[x + "_scale"][b, h].double()[:, None]
+
+        for h in range(Hkv):
+            kp, vp = (head(st["prefix"], x, None, h) for x in "kv")
+            for b, L in enumerate(_lengths(c)):
+                ks = torch.cat([kp, head(st["own"], "k", b, h)[:L]])
+                vs = torch.cat([vp, head(st["own"], "v", b, h)[:L]])
+                if not len(ks):
+                    continue
+                for g in range(Hq // Hkv):
+                    j = h * (Hq // Hkv) + g
+                    s = (st["q"][b, j].double() @ ks.T) / math.sqrt(d)
+                    if c["causal"]:
+                        i = torch.arange(n, device=DEV)[:, None]
+                        s = s.masked_fill(torch.arange(len(ks), device=DEV)[None] >= P + (L - n + 1 + i).clamp_min(0), -math.inf)
+                    res[b, :, j] = torch.nan_to_num(torch.softmax(s, -1), nan=0.0) @ vs
+        return res.reshape(B, n, Hq * d)
+    # group normalisation: the formula and its derivative by torch in 64 bits
+    train = c["op"] == "gn_train"
+    x, wt, bs = (st[k].detach().double().requires_grad_(train) for k in ("x", "weight", "bias"))
+    parts = x.reshape(c["B"], c["G"], -1)
+    var, mu = torch.var_mean(parts, -1, unbiased=False, keepdim=True)
+    z = ((parts - mu) / torch.sqrt(var + 1e-5)).reshape(x.shape) * wt[:, None, None] + bs[:, None, None]
+    y = z * torch.sigmoid(z) if c["act"] == "silu" else z
+    if not train:
+        return y
+    return (y.detach(),) + torch.autograd.grad(y, (x, wt, bs), st["dy"].double())
