@@ -143,10 +143,11 @@ def _quantise(rows, fmt):
     top = _TOP[fmt]
     amax = x.abs().amax(-1, keepdim=True)
     live = amax >= _TINY
-    inv = torch.where(live, top / torch.where(live, amax, 1.0), 0.0)
+    most = torch.full_like(amax, top)          # a tensor: torch divides by a number through its reciprocal
+    inv = torch.where(live, most / torch.where(live, amax, 1.0), 0.0)
     y = (x * inv).clamp(-top, top)
     codes = torch.round(y).to(torch.int8) if fmt == "int8" else y.to(torch.float8_e4m3fn)
-    return codes, torch.where(live, amax / top, 0.0).squeeze(-1)
+    return codes, torch.where(live, amax / most, 0.0).squeeze(-1)
 
 
 def _plain_write(st):
