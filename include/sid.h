@@ -35,6 +35,7 @@ extern "C" {
 /* storage type of the q/k/v/out tensors */
 #define SID_DTYPE_F32 0
 #define SID_DTYPE_BF16 1
+#define SID_DTYPE_F16 2 /* the 8-bit cache, shared-prefix attention and group norm; the other entry points refuse it */
 
 /* arithmetic of the two matrix products inside the attention kernels */
 #define SID_COMPUTE_BF16 0  /* bf16 MFMA operands, f32 accumulate: <= 2e-2 relative at unit-variance q, k (see F16QK) */
@@ -84,6 +85,15 @@ extern "C" {
 #define SID_FLAG_STAGE_PACK 0x10
 #define SID_FLAG_STAGE_FLASH 0x20
 #define SID_FLAG_STAGE_MERGE 0x40
+
+/* activations fused into the group norm */
+#define SID_ACT_NONE 0
+#define SID_ACT_SILU 1
+
+/* how a cache holds keys and values */
+#define SID_KV_NONE 0 /* 16-bit tensors of the call's type */
+#define SID_KV_INT8 1 /* 8-bit integers in [-127, 127] and one f32 scale per row */
+#define SID_KV_E4M3 2 /* 8-bit floats (e4m3, largest 448) and one f32 scale per row */
 
 const char* sid_last_error(void);
 int sid_version(void);
@@ -314,6 +324,87 @@ int sid_residual_sum(const void* skip, const void* h, const void* hf, void* out,
  */
 int sid_masked_adain(const void* cnt, const void* sty_char, const void* sty_back, const float* mask,
                      int Hin, int Win, void* out, int B, int C, int H, int W, int dtype, void* stream);
+
+/*
+ * Key/value cache in 8 bits.  No counterpart in the reference, whose feature store keeps fp32 tensors
+ * (run_ori.py:168-222).
+ *
+ * A cache of B sequences holds codes (B, H, S, d), one byte each, and scales (B, H, S) in f32, for keys and for
+ * values; all contiguous.  A code stands for code * scale.  head_dim d: a multiple of 8 in [8, 256].
+ *
+ *   sid_kv_cache_write   rows i < n of sequence b, k and v (B, H, n, d), go to positions start[b] + i.  A row gets
+ *                        scale = amax / top and codes round_to_nearest_even(x * (top / amax)), top = 127 (int8) or 448
+ *                        (e4m3), in f32.  amax < 2^-100: zeros with scale 0; an infinity or NaN in the row: scale NaN
+ *                        (the row reads back as NaN).  Rows with i >= length[b] and positions outside [0, S) are
+ *                        skipped; everything that is not written stays as it was.
+ *   sid_kv_cache_read    the n positions from start[b] on, as numbers of `dtype`: k, v (B, H, n, d) contiguous.
+ *                        Positions outside [0, S) give zeros.
+ *
+ *   k_strides, v_strides  HOST arrays of three: elements from sequence to sequence, head to head, token to token (the
+ *                         last dimension is contiguous); rows 16-byte aligned.
+ *   start                 (B) int32 on the device;  length: (B) int32 on the device, or NULL: n for all.
+ */
+int sid_kv_cache_write(const void* k, const void* v, const long long* k_strides, const long long* v_strides,
+                       void* k_codes, void* v_codes, float* k_scale, float* v_scale,
+                       const int* start, const int* length,
+                       int B, int H, int n, int S, int d, int dtype, int fmt, void* stream);
+
+int sid_kv_cache_read(const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale,
+                      void* k, void* v, const int* start,
+                      int B, int H, int n, int S, int d, int dtype, int fmt, void* stream);
+
+/*
+ * Attention of a batch that shares a prefix of keys and values.
+ * The reference's single-style path repeats the injected keys and values for every image of a batch
+ * (ldm/modules/attention.py:389-401, torch.cat([k_injected] * b)); here the prefix exists once.
+ *
+ *   q         (B, Hq, n, d)        out  (B, n, Hq*d) contiguous      bf16 or f16
+ *   prefix    P keys and values (Hkv, P, d), one copy for the batch     (P = 0: may be NULL)
+ *   own       S keys and values per sequence (B, Hkv, S, d)             (S = 0: may be NULL)
+ *   own_len   (B) int32 on the device: sequence b has its first own_len[b] own keys (clamped to [0, S]); NULL: all S
+ *   causal    not 0: query i sees its own keys j <= own_len[b] - n + i (the last query sees all of them)
+ *
+ * Query head h reads key/value head h / (Hq / Hkv).  One softmax over scale * q.k of the prefix and the own keys that a
+ * query sees, in f32; a query that sees none gives zeros.  Keys behind own_len are never read into the result,
+ * whatever they hold.  Products run at 16-bit operands (8-bit codes become numbers of `dtype` first), probabilities are
+ * rounded to `dtype` for the second product.  A query that sees a non-finite value within 64 keys of the causal edge
+ * comes out NaN in all its columns (elsewhere: in the columns of that value).
+ * scale: positive and finite.
+ */
+typedef struct sid_kv_source {
+    const void *k, *v;                 /* 16-bit numbers (fmt SID_KV_NONE) or codes */
+    const float *k_scale, *v_scale;    /* 8-bit formats: one per row, rows contiguous; else NULL */
+    long long k_stride[3], v_stride[3];/* elements from sequence to sequence (unused for a prefix), head to head, token to token */
+    long long scale_stride[2];         /* scales from sequence to sequence, head to head */
+    int fmt;
+} sid_kv_source;
+
+size_t sid_shared_attn_workspace_bytes(int B, int Hq, int Hkv, int n, int d, int P, int S);
+
+int sid_shared_attn_fwd(const void* q, const long long* q_stride, const sid_kv_source* prefix, const sid_kv_source* own,
+                        const int* own_len, void* out, int B, int Hq, int Hkv, int n, int d, int P, int S,
+                        float scale, int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Group normalisation with an activation, channels last.
+ * Stands for GroupNorm32 + SiLU of the host network's ResBlocks (ldm/modules/diffusionmodules/openaimodel.py:219-263) and
+ * the GroupNorm of SpatialTransformer (ldm/modules/attention.py:695-717), on tensors with the channels contiguous.
+ *   x, y, dy, dx  (B, N, C), C contiguous (an NCHW tensor in channels-last memory has N = H*W)
+ *   weight, bias  (C) f32, either may be NULL (ones / zeros)
+ *   mean, rstd    (B, G) f32: written by the forward, read by the backward
+ *   y = act((x - mean) * rstd * weight + bias), biased variance, statistics in f32
+ *   dweight, dbias  (C) f32 sums over the batch, either may be NULL.  Results repeat bit for bit (no atomics).
+ */
+size_t sid_group_norm_workspace_bytes(int B, int N, int C, int G, int dtype, int backward);
+
+int sid_group_norm_act_fwd(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd,
+                           int B, int N, int C, int G, float eps, int act, int dtype,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+int sid_group_norm_act_bwd(const void* dy, const void* x, const float* weight, const float* bias,
+                           const float* mean, const float* rstd, void* dx, float* dweight, float* dbias,
+                           int B, int N, int C, int G, int act, int dtype,
+                           void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1348,6 +1348,11 @@ int launch_flash_nw(const FlashParams& fp, const Geometry& g, hipStream_t stream
     }
 }
 
+// The widest class (head_dim 145-160) is instantiated in sid_attn_wide.hip, which is compiled with a scheduler of its own.
+extern template int launch_flash_nw<10, 6, false, false, false>(const FlashParams&, const Geometry&, hipStream_t);
+extern template int launch_flash_nw<10, 6, false, false, true>(const FlashParams&, const Geometry&, hipStream_t);
+extern template int launch_flash_nw<10, 6, true, false, false>(const FlashParams&, const Geometry&, hipStream_t);
+
 // The half-precision logits mode is instantiated for every head-dim class the bf16 mode serves.
 constexpr bool f16qk_instance(int DKS, int DVB) { return DKS > 0 && DVB > 0; }
 

@@ -1,0 +1,174 @@
+// Shared-prefix attention: decomposition, the joining kernel and the entry points.  Kernels: sid_shared_kernel.hpp.
+#include "sid_shared_kernel.hpp"
+
+#include <cmath>
+
+namespace sid_shared {
+namespace {
+
+// out = sum over slots of 2^(m - M) part / sum of 2^(m - M) l.  One thread per four columns of a row.
+template <typename T>
+__global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ part, const float2* __restrict__ stats, char* __restrict__ out,
+                                                      long long rows, int d, int slots) {
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int quads = d / 4;
+    const long long row = id / quads;
+    if (row >= rows) return;
+    const int c = (int)(id - row * quads) * 4;
+    float top = kNegInf;
+    for (int s = 0; s < slots; ++s) top = fmaxf(top, stats[(long long)s * rows + row].x);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    float total = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < slots; ++s) {
+        const float2 st = stats[(long long)s * rows + row];
+        const float4 o = *(const float4*)(part + ((long long)s * rows + row) * d + c);
+        // an empty slot has reference -inf and sum 0; one whose keys gave NaN may have that reference and a NaN sum
+        const float w = st.x == kNegInf ? (st.y == 0.f ? 0.f : st.y) : __builtin_amdgcn_exp2f(st.x - top);
+        total = __builtin_fmaf(w, st.y, total);
+        a.x = __builtin_fmaf(w, o.x, a.x); a.y = __builtin_fmaf(w, o.y, a.y);
+        a.z = __builtin_fmaf(w, o.z, a.z); a.w = __builtin_fmaf(w, o.w, a.w);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    store4<T>(out + (row * d + c) * 2, a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+}
+
+struct Plan {
+    int qt, slots;
+    unsigned grid;
+    Group g[2];
+    int blocks0;
+};
+
+constexpr int kFill = 512;          // workgroups that fill the chip: two on each of 256 CUs
+
+int padded(int items) { return (items + kXcd - 1) / kXcd * kXcd; }
+int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// Splits of a key range of `keys` so that `items` x splits workgroups fill the chip, each with at least `least` keys.
+int splits_for(long long items, long long keys, int least) {
+    long long s = (kFill + items - 1) / items;
+    if (s > keys / least) s = keys / least;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+Plan make_plan(int B, int Hkv, int G, int n, int d, int P, int S) {
+    Plan pl{};
+    const long long rows = (long long)n * G;             // of one image
+    pl.qt = 1;
+    auto add = [&](int k, int tiles, int tile_rows, int splits, int per_image, int by_keys, int segs) {
+        pl.g[k] = Group{(int)((long long)Hkv * (per_image ? B : 1) * tiles * splits), tiles, splits, pl.slots, tile_rows, per_image, by_keys, segs};
+        pl.slots += splits;
+    };
+    if (rows > 64) {
+        // many rows per image: each tile walks prefix and own keys
+        pl.qt = two_tiles(class_of(d)) && rows > 128 ? 2 : 1;
+        const int tile = 128 * pl.qt, tiles = ceil_div(rows, tile);
+        add(0, tiles, tile, splits_for((long long)B * Hkv * tiles, (long long)P + S, 512), 1, 0, (P ? 1 : 0) | (S ? 2 : 0));
+    } else {
+        int k = 0;
+        if (P) {
+            const long long all = rows * B;
+            const int by_keys = all <= 32, tile = by_keys ? 32 : 128, tiles = ceil_div(all, tile);
+            add(k++, tiles, tile, splits_for((long long)Hkv * tiles, P, 256), 0, by_keys, 1);
+        }
+        if (S) {
+            const int tiles = ceil_div(rows, 32);
+            add(k++, tiles, 32, splits_for((long long)B * Hkv * tiles, S, 256), 1, 1, 2);
+        }
+        if (!k) add(0, ceil_div(rows, 32), 32, 1, 1, 1, 0);          // no keys at all: zeros
+    }
+    pl.blocks0 = padded(pl.g[0].items);
+    pl.grid = (unsigned)(pl.blocks0 + padded(pl.g[1].items));
+    return pl;
+}
+
+int check_shape(int B, int Hq, int Hkv, int n, int d, int P, int S) {
+    SID_CHECK_ARG(B >= 1 && Hq >= 1 && Hkv >= 1 && n >= 1, "B, heads and queries must be >= 1");
+    SID_CHECK_ARG(P >= 0 && S >= 0, "key counts must not be negative");
+    SID_CHECK_ARG(Hq % Hkv == 0, "%d query heads do not divide among %d key/value heads", Hq, Hkv);
+    SID_CHECK_ARG(d >= 8 && d <= 256 && d % 8 == 0, "head_dim must be a multiple of 8 in [8, 256], got %d", d);
+    SID_CHECK_ARG((long long)B * n * Hq < (1 << 24) && P < (1 << 30) && S < (1 << 30), "too many rows or keys");
+    return SID_OK;
+}
+
+size_t plan_bytes(const Plan& pl, long long rows, int d) {
+    return pl.slots <= 1 ? 0 : sid::align_up((size_t)pl.slots * rows * d * 4, 256) + (size_t)pl.slots * rows * sizeof(float2);
+}
+
+int check_source(const sid_kv_source* s, int keys, int d, const char* what) {
+    SID_CHECK_ARG(s && s->k && s->v, "%s: NULL pointer", what);
+    SID_CHECK_ARG(s->fmt == SID_KV_NONE || s->fmt == SID_KV_INT8 || s->fmt == SID_KV_E4M3, "%s: unknown format %d", what, s->fmt);
+    const int es = s->fmt == SID_KV_NONE ? 2 : 1, unit = s->fmt == SID_KV_NONE ? 16 : 8;
+    const long long st[6] = {s->k_stride[0], s->k_stride[1], s->k_stride[2], s->v_stride[0], s->v_stride[1], s->v_stride[2]};
+    SID_CHECK_ARG((uintptr_t)s->k % unit == 0 && (uintptr_t)s->v % unit == 0, "%s: keys and values must be %d-byte aligned", what, unit);
+    for (long long x : st) SID_CHECK_ARG(x * es % unit == 0, "%s: rows must be %d-byte aligned", what, unit);
+    for (int i = 2; i < 6; i += 3)
+        SID_CHECK_ARG(st[i] >= 0 && st[i] * es < (1 << 24), "%s: distance between tokens out of range", what);
+    if (s->fmt != SID_KV_NONE) SID_CHECK_ARG(s->k_scale && s->v_scale, "%s: scales missing", what);
+    return SID_OK;
+}
+
+void fill_source(Source& o, const sid_kv_source* s) {
+    const int es = s->fmt == SID_KV_NONE ? 2 : 1;
+    o.k = (const char*)s->k; o.v = (const char*)s->v;
+    o.ks = s->k_scale; o.vs = s->v_scale;
+    o.kb = s->k_stride[0] * es; o.kh = s->k_stride[1] * es; o.kn = (int)(s->k_stride[2] * es);
+    o.vb = s->v_stride[0] * es; o.vh = s->v_stride[1] * es; o.vn = (int)(s->v_stride[2] * es);
+    o.sb = s->scale_stride[0]; o.sh = s->scale_stride[1];
+    o.fmt = s->fmt;
+}
+
+}  // namespace
+}  // namespace sid_shared
+
+using namespace sid_shared;
+
+extern "C" size_t sid_shared_attn_workspace_bytes(int B, int Hq, int Hkv, int n, int d, int P, int S) {
+    if (check_shape(B, Hq, Hkv, n, d, P, S)) return 0;
+    const size_t need = plan_bytes(make_plan(B, Hkv, Hq / Hkv, n, d, P, S), (long long)B * n * Hq, d);
+    return need ? need : 256;
+}
+
+extern "C" int sid_shared_attn_fwd(const void* q, const long long* q_stride, const sid_kv_source* prefix, const sid_kv_source* own,
+                                   const int* own_len, void* out, int B, int Hq, int Hkv, int n, int d, int P, int S,
+                                   float scale, int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    SID_CHECK_ARG(q && q_stride && out, "NULL pointer");
+    if (int rc = check_shape(B, Hq, Hkv, n, d, P, S)) return rc;
+    SID_CHECK_ARG(dtype == SID_DTYPE_BF16 || dtype == SID_DTYPE_F16, "queries must be bf16 or f16, got dtype %d", dtype);
+    SID_CHECK_ARG(scale > 0.f && std::isfinite(scale), "scale must be positive and finite");
+    SID_CHECK_ARG((uintptr_t)q % 16 == 0 && (uintptr_t)out % 8 == 0, "queries must be 16-byte aligned, the output 8-byte");
+    for (int i = 0; i < 3; ++i) SID_CHECK_ARG(q_stride[i] % 8 == 0, "query rows must be 16-byte aligned");
+    if (P) if (int rc = check_source(prefix, P, d, "prefix")) return rc;
+    if (S) if (int rc = check_source(own, S, d, "own part")) return rc;
+
+    const Plan pl = make_plan(B, Hkv, Hq / Hkv, n, d, P, S);
+    const long long rows = (long long)B * n * Hq;
+    const size_t need = plan_bytes(pl, rows, d);
+    if (need > workspace_bytes) return sid::fail(SID_ENOMEM, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    SID_CHECK_ARG(need == 0 || (workspace && (uintptr_t)workspace % 256 == 0), "workspace must be 256-byte aligned");
+    Params p{};
+    p.q = (const char*)q;
+    p.qb = q_stride[0] * 2; p.qh = q_stride[1] * 2; p.qn = q_stride[2] * 2;
+    if (P) fill_source(p.src[0], prefix);
+    if (S) fill_source(p.src[1], own);
+    p.own_len = own_len;
+    p.out = (char*)out;
+    if (need) {
+        p.part = (float*)workspace;
+        p.stats = (float2*)((char*)workspace + sid::align_up((size_t)pl.slots * rows * d * 4, 256));
+    }
+    p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.n = n; p.d = d; p.P = P; p.S = S; p.causal = causal != 0;
+    p.c = scale * 1.4426950408889634f;
+    p.blocks0 = pl.blocks0;
+    p.g[0] = pl.g[0]; p.g[1] = pl.g[1];
+    const hipStream_t st = (hipStream_t)stream;
+    if (int rc = dtype == SID_DTYPE_BF16 ? launch_bf16(p, pl.qt, pl.grid, st) : launch_f16(p, pl.qt, pl.grid, st)) return rc;
+    if (need) {
+        const unsigned grid = (unsigned)((rows * (d / 4) + 255) / 256);
+        if (dtype == SID_DTYPE_BF16) hipLaunchKernelGGL(combine_kernel<__bf16>, dim3(grid), dim3(256), 0, st, p.part, p.stats, p.out, rows, d, pl.slots);
+        else hipLaunchKernelGGL(combine_kernel<_Float16>, dim3(grid), dim3(256), 0, st, p.part, p.stats, p.out, rows, d, pl.slots);
+        SID_CHECK_HIP(hipGetLastError());
+    }
+    return SID_OK;
+}

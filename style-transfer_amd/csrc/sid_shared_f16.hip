@@ -1,0 +1,6 @@
+// Half-precision instances of the shared-prefix attention kernels.
+#include "sid_shared_kernel.hpp"
+
+namespace sid_shared {
+int launch_f16(const Params& p, int qt, unsigned grid, hipStream_t st) { return launch_type<_Float16>(p, qt, grid, st); }
+}  // namespace sid_shared

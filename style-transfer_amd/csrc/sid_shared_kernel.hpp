@@ -1,0 +1,624 @@
+// Attention of a batch whose sequences share a prefix of keys and values: device code and launch templates.
+//
+// Row r = (b n + i) G + g of key/value head h is query i of head h G + g of image b.  It attends to the P keys of the
+// prefix (one copy for the whole batch) and to the first lim(r) of its image's own S keys under one softmax:
+//   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  s_j = scale q.k_j,
+// lim = own_len[b], or with the causal order min(own_len, max(0, own_len - n + 1 + i)).  A row without keys gives zeros.
+//
+// Work items.  An item is a tile of rows times a range of key tiles; it yields the un-normalised output, the softmax
+// reference and the row sum, which combine_kernel joins when a row has more than one.
+//   Many rows per image: items are row tiles of one image and walk the prefix, then the own keys.
+//   Few rows per image (decoding): the rows of ALL images that share a key/value head stand in the same tiles against the
+//   prefix, so the prefix is read once for the batch and not once per image; the own keys are items of their own.
+//   Long key ranges are split over items until the chip is full.
+//
+// Two ways for a workgroup of four waves to share an item:
+//   rows   each wave owns 32 QT rows, key tiles of 64 are staged for all four (double-buffered, one barrier a tile);
+//   keys   up to 32 rows: every wave takes every fourth tile of 32 keys through its own buffer, without barriers, and
+//          the four results are joined at the end.  One row (a single token) costs the matrix unit as much as 32, which
+//          is still below the time that the keys take to arrive.
+//
+// MFMA 32x32x16, keys on rows and queries on lanes as in sid_attn_kernel.hpp: S^T = K Q^T, whose accumulator rounded to
+// 16 bits is the B operand of O^T += V^T P^T when the key order of the A operand follows the accumulator's.  V stays
+// row-major in LDS; ds_read_b64_tr_b16 hands every lane four consecutive keys of its column.  Where head_dim leaves a
+// spare column in V's last block of 32, that column holds ones and the product also yields the row sum.
+// Tiles go through registers to LDS: the next tile's loads are in flight while this one is computed, and keys behind the
+// end become zeros.  8-bit codes become the call's 16-bit type on the way: key codes as they are (both types hold them
+// exactly; their scale multiplies the f32 logits, because a rounding of the keys would shift a logit by 2^-9 of the sum of
+// |q k|, twice the error of everything else at |logit| = 5), value codes times their scale, rounded once.
+#pragma once
+#include "sid_common.h"
+
+#include <cstdint>
+
+namespace sid_shared {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+
+constexpr int kXcd = 8;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+struct Source {                      // keys and values of the prefix, or of the images' own part
+    const char *k, *v;
+    const float *ks, *vs;            // 8-bit formats: one scale per row
+    long long kb, kh, vb, vh;        // bytes from image to image, head to head
+    long long sb, sh;                // the same for the scales, in floats
+    int kn, vn;                      // bytes from key to key
+    int fmt;                         // SID_KV_NONE: the call's 16-bit type
+};
+
+struct Group {                       // work items of one kind
+    int items, tiles, splits, slot0, tile_rows;
+    int per_image;                   // row tiles of one image, or of all images together
+    int keys_way;                    // waves share the keys (up to 32 rows) instead of the rows
+    int segs;                        // 1: prefix, 2: own, 3: both
+};
+
+struct Params {
+    const char* q;
+    long long qb, qh, qn;            // strides in bytes
+    Source src[2];                   // prefix, own
+    const int* own_len;
+    char* out;                       // (B, n, Hq, d)
+    float* part;                     // [slot][B n Hq][d], or null: one item per row, which writes `out`
+    float2* stats;                   // [slot][B n Hq]: softmax reference (log2 domain), row sum; 0 = nothing in it
+    int B, Hq, Hkv, G, n, d, P, S, causal;
+    float c;                         // scale * log2(e)
+    int blocks0;                     // workgroups of group 0 (a multiple of 8)
+    Group g[2];
+};
+
+template <typename T> struct Ops;
+template <> struct Ops<__bf16> {
+    using V8 = bf16x8;
+    static constexpr uint16_t kExp = 0x7f80, kOne = 0x3f80;
+    static constexpr float kBias = 0.f;
+    static __device__ __forceinline__ f32x16 mfma(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Ops<_Float16> {
+    using V8 = f16x8;
+    static constexpr uint16_t kExp = 0x7c00, kOne = 0x3c00;
+    // probabilities reach 2^(8 + 6), inside half's range; the smallest it can tell from zero is 2^-30 of the largest
+    static constexpr float kBias = 6.f;
+    static __device__ __forceinline__ f32x16 mfma(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+
+// The head-dim classes: KS steps of 16 in q.k, DVB blocks of 32 in V, LPR lanes that stage one row (8 elements each).
+template <int KS> struct Dims {
+    static constexpr int DVB = (KS + 1) / 2;
+    static constexpr int LPR = KS <= 4 ? 8 : KS <= 8 ? 16 : 32;
+    static constexpr int KSTR = KS * 16 + 8, VSTR = DVB * 32 + 8;        // LDS row strides in elements (pads spread banks)
+    static constexpr int KELEMS = 128 * KSTR, VELEMS = 128 * VSTR;       // 128 rows: 2 x 64 (rows way) = 4 x 32 (keys way)
+    static constexpr int MSTR = DVB * 32 + 4;                            // joining four waves: [4][32][MSTR] floats
+    static constexpr size_t kStage = (size_t)(KELEMS + VELEMS) * 2;
+    static constexpr size_t kJoin = (size_t)(4 * 32 * MSTR + 2 * 4 * 32) * 4;
+    static constexpr size_t kRowData = kStage > kJoin ? kStage : kJoin;              // then per key row a scale and a flag
+    static constexpr size_t kLds = kRowData + 128 * 8;
+    static constexpr int NS = KS <= 10 ? 2 : 1;      // sub-tiles of 32 keys whose logits are in registers together
+    static constexpr bool kAhead = KS <= 10;         // a tile waits in registers while the one before it is computed
+};
+
+// One key tile on its way from memory to LDS.  NT threads, KT keys.
+template <typename T, int KS, int NT, int KT>
+struct Stager {
+    using D = Dims<KS>;
+    static constexpr int RPP = NT / D::LPR, NJ = KT / RPP;
+    uint4 k[NJ], v[NJ];
+    int fmt;
+
+    __device__ __forceinline__ void load(const Params& p, int seg, int b, int h, int key0, int end, int t) {
+        const Source& s = p.src[seg];
+        fmt = s.fmt;
+        const int col = t % D::LPR, row = t / D::LPR;
+        const bool live = col * 8 < p.d;
+        const int bi = seg ? b : 0;
+        const int step = s.fmt == SID_KV_NONE ? 16 : 8;
+        const char* kp = s.k + bi * s.kb + h * s.kh + (long long)key0 * s.kn;
+        const char* vp = s.v + bi * s.vb + h * s.vh + (long long)key0 * s.vn;
+        if (s.fmt == SID_KV_NONE) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int r = row + j * RPP;
+                k[j] = v[j] = make_uint4(0u, 0u, 0u, 0u);
+                if (live && key0 + r < end) {
+                    k[j] = *(const uint4*)(kp + (unsigned)(r * s.kn + col * step));
+                    v[j] = *(const uint4*)(vp + (unsigned)(r * s.vn + col * step));
+                }
+            }
+        } else {
+            const float* ks = s.ks + bi * s.sb + h * s.sh + key0;
+            const float* vs = s.vs + bi * s.sb + h * s.sh + key0;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int r = row + j * RPP;
+                k[j] = v[j] = make_uint4(0u, 0u, 0u, 0u);
+                if (live && key0 + r < end) {
+                    const uint2 a = *(const uint2*)(kp + (unsigned)(r * s.kn + col * step));
+                    const uint2 c = *(const uint2*)(vp + (unsigned)(r * s.vn + col * step));
+                    k[j] = make_uint4(a.x, a.y, __float_as_uint(ks[r]), 0u);
+                    v[j] = make_uint4(c.x, c.y, __float_as_uint(vs[r]), 0u);
+                }
+            }
+        }
+    }
+
+    // eight codes as numbers of type T, times `scale`
+    static __device__ __forceinline__ uint4 numbers(uint4 a, int fmt, float scale) {
+        float f[8];
+        const uint32_t w[2] = {a.x, a.y};
+        if (fmt == SID_KV_INT8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(w[e / 4] >> (8 * (e & 3)));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[e], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[e], true);
+                f[4 * e] = lo[0]; f[4 * e + 1] = lo[1]; f[4 * e + 2] = hi[0]; f[4 * e + 3] = hi[1];
+            }
+        }
+        typename Ops<T>::V8 o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = (T)(f[e] * scale);
+        return __builtin_bit_cast(uint4, o);
+    }
+
+    // `edge`: keys that some rows of the tile do not see are in it.  Their probability is zero, but zero times an
+    // infinity or a NaN is not: such values become zeros and the key is flagged (rows that do see it turn NaN).
+    __device__ __forceinline__ void store(const Params& p, T* kl, T* vl, float* scale, bool edge, int* bad, int t) {
+        const int col = t % D::LPR, row = t / D::LPR;
+        if (col * 8 >= p.d) return;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int r = row + j * RPP;
+            uint4 a = k[j], c = v[j];
+            if (fmt != SID_KV_NONE) {
+                if (col == 0) scale[r] = __uint_as_float(a.z) * p.c;
+                a = numbers(a, fmt, 1.f);
+                c = numbers(c, fmt, __uint_as_float(c.z));
+            }
+            if (edge) {
+                uint32_t w[4] = {c.x, c.y, c.z, c.w};
+                bool any = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t E = Ops<T>::kExp;
+                    if ((w[e] & E) == E) { w[e] &= 0xffff0000u; any = true; }
+                    if ((w[e] & (E << 16)) == (E << 16)) { w[e] &= 0xffffu; any = true; }
+                }
+                c = make_uint4(w[0], w[1], w[2], w[3]);
+                if (any) bad[r] = 1;
+            }
+            *(uint4*)(kl + r * D::KSTR + col * 8) = a;
+            *(uint4*)(vl + r * D::VSTR + col * 8) = c;
+        }
+    }
+};
+
+// Softmax state of QT tiles of 32 queries (one query per lane pair) and their output accumulators.
+template <typename T, int KS, int QT, bool ONES>
+struct Rows {
+    using D = Dims<KS>;
+    using V8 = typename Ops<T>::V8;
+    V8 q[QT][KS];
+    f32x16 o[QT][D::DVB];
+    float m[QT], l[QT];              // softmax reference (log2 domain); row sum of this lane's keys (unless ONES)
+    int lim[QT];                     // own keys that the row sees
+
+    __device__ __forceinline__ void init(const Params& p, int h, int row_begin, int row_end, int lane, int L) {
+        const int r32 = lane & 31, hi = lane >> 5;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int r = row_begin + t * 32 + r32;
+            const bool in = r < row_end;
+            const int tok = in ? r / p.G : 0, g = in ? r - tok * p.G : 0, b = tok / p.n, i = tok - b * p.n;
+            const char* src = p.q + b * p.qb + (long long)(h * p.G + g) * p.qh + i * p.qn;
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) {
+                const int e = kk * 16 + hi * 8;
+                q[t][kk] = in && e < p.d ? *(const V8*)(src + e * 2) : V8{};
+            }
+            lim[t] = !in ? 0x7fffffff : p.causal ? min(L, max(0, L - p.n + 1 + i)) : L;
+            m[t] = kNegInf;
+            l[t] = 0.f;
+#pragma unroll
+            for (int d = 0; d < D::DVB; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[t][d][e] = 0.f;
+        }
+    }
+
+    // NS sub-tiles of 32 keys in LDS; `scaled`: every key's logits carry its own factor; `masked`: some row sees only the keys
+    // below its own part's limit (seg), or below P.
+    template <int NS>
+    __device__ __forceinline__ void tile(const Params& p, const T* kl, const T* vl, const float* scale, bool scaled, int seg, int key0, bool masked, bool edge,
+                                         const int* bad, int lane) {
+        const int r32 = lane & 31, hi = lane >> 5;
+        f32x16 s[QT][NS];
+#pragma unroll
+        for (int u = 0; u < NS; ++u) {
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[t][u][e] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) {
+                const V8 a = *(const V8*)(kl + (u * 32 + r32) * D::KSTR + kk * 16 + hi * 8);
+#pragma unroll
+                for (int t = 0; t < QT; ++t) s[t][u] = Ops<T>::mfma(a, q[t][kk], s[t][u]);
+            }
+        }
+        const float c = scaled ? 1.f : p.c;
+        if (scaled) {
+#pragma unroll
+            for (int u = 0; u < NS; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float4 f = *(const float4*)(scale + u * 32 + 2 * e + 4 * hi);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) { s[t][u][e] *= f.x; s[t][u][e + 1] *= f.y; s[t][u][e + 2] *= f.z; s[t][u][e + 3] *= f.w; }
+                }
+        }
+        if (masked) {
+#pragma unroll
+            for (int u = 0; u < NS; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int key = u * 32 + 8 * (e >> 2) + 4 * hi + (e & 3);
+                    const bool poison = edge && bad[key];
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) {
+                        if (poison) s[t][u][e] = __builtin_nanf("");
+                        if (key0 + key >= (seg ? lim[t] : p.P)) s[t][u][e] = kNegInf;
+                    }
+                }
+        }
+        V8 pr[QT][NS][2];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            float mt = s[t][0][0];
+#pragma unroll
+            for (int u = 0; u < NS; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[t][u][e]);
+            mt = fmaxf(mt, other_half(mt)) * c;
+            // the reference moves only when a logit exceeds it by 2^8: probabilities stay below that, nothing overflows
+            const bool up = mt - m[t] > 8.f || (m[t] == kNegInf && mt > kNegInf);
+            if (__any(up)) {
+                const float mn = up ? mt : m[t];
+                const float alpha = m[t] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[t] - mn);
+                m[t] = mn;
+                l[t] *= alpha;
+#pragma unroll
+                for (int d = 0; d < D::DVB; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[t][d][e] *= alpha;
+            }
+            const float off = m[t] == kNegInf ? 0.f : Ops<T>::kBias - m[t];
+#pragma unroll
+            for (int u = 0; u < NS; ++u) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[t][u][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][u][e], c, off));
+                if (!ONES)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) l[t] += s[t][u][e];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) pr[t][u][e >> 3][e & 7] = (T)s[t][u][e];
+            }
+        }
+        // V^T fragments: lane 16 a + x of a half reads row x / 4, columns 4 (x % 4) .. of a block of 4 keys and 16 columns
+        const int x = lane & 15;
+        const T* vb = vl + (4 * hi + (x >> 2)) * D::VSTR + ((lane >> 4) & 1) * 16 + (x & 3) * 4;
+#pragma unroll
+        for (int u = 0; u < NS; ++u)
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int d = 0; d < D::DVB; ++d) {
+                    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+                    const T* at = vb + (u * 32 + w * 16) * D::VSTR + d * 32;
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at);
+                    const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 8 * D::VSTR));
+                    const V8 a = __builtin_bit_cast(V8, __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) o[t][d] = Ops<T>::mfma(a, pr[t][u][w], o[t][d]);
+                }
+    }
+
+    __device__ __forceinline__ float row_sum(const Params& p, int t) const {
+        float sum = l[t];
+        if (ONES) {
+            // column d of V: block d / 32, register 4 ((d % 32) / 8), lower half (d is a multiple of 8)
+#pragma unroll
+            for (int d = 0; d < D::DVB; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) sum = d * 32 + 2 * e == p.d ? o[t][d][e] : sum;
+            const float low = other_half(sum);
+            return (threadIdx.x & 32) ? low : sum;
+        }
+        return sum + other_half(sum);
+    }
+    __device__ __forceinline__ float reference(const Params& p, int t) const { return m[t] == kNegInf ? kNegInf : m[t] - Ops<T>::kBias; }
+};
+
+template <typename T>
+__device__ __forceinline__ void store4(char* p, float a, float b, float c, float d) {
+    typedef __attribute__((ext_vector_type(4))) T T4;
+    T4 v;
+    v[0] = (T)a; v[1] = (T)b; v[2] = (T)c; v[3] = (T)d;
+    *(T4*)p = v;
+}
+
+struct Item { int h, b, row_begin, row_end, L, TP, v0, v1, slot; };
+
+// Key range of the item in tiles of KT keys: first the prefix's, then the own ones.
+__device__ __forceinline__ bool find_item(const Params& p, Item& it, bool& keys_way) {
+    const bool second = (int)blockIdx.x >= p.blocks0;
+    const Group& g = p.g[second];
+    const int i = (int)blockIdx.x - (second ? p.blocks0 : 0), share = (g.items + kXcd - 1) / kXcd;
+    // workgroup i runs on XCD i mod 8: every XCD takes a contiguous share of the items, which share keys through its L2
+    int w = (i % kXcd) * share + i / kXcd;
+    if (w >= g.items || i / kXcd >= share) return false;
+    keys_way = g.keys_way;
+    const int tile = w % g.tiles;
+    w /= g.tiles;
+    const int split = w % g.splits;
+    w /= g.splits;
+    it.b = g.per_image ? w % p.B : 0;
+    it.h = g.per_image ? w / p.B : w;
+    const int rows = p.n * p.G, first = g.per_image ? it.b * rows : 0, last = g.per_image ? first + rows : p.B * rows;
+    it.row_begin = first + tile * g.tile_rows;
+    it.row_end = min(last, it.row_begin + g.tile_rows);
+    const int KT = g.keys_way ? 32 : 64;
+    it.TP = (g.segs & 1) ? (p.P + KT - 1) / KT : 0;
+    it.L = 0;
+    int TO = 0;
+    if (g.segs & 2) {
+        it.L = p.own_len ? min(max(p.own_len[it.b], 0), p.S) : p.S;
+        int most = it.L;
+        if (p.causal) most = min(most, max(0, it.L - p.n + 1 + (it.row_end - 1 - first) / p.G));
+        TO = (most + KT - 1) / KT;
+    }
+    const long long TT = it.TP + TO;
+    it.v0 = (int)(TT * split / g.splits);
+    it.v1 = (int)(TT * (split + 1) / g.splits);
+    it.slot = g.slot0 + split;
+    return true;
+}
+
+// Zeros everywhere (the pads behind head_dim are never written again), ones in the spare column.
+template <typename T, int KS, bool ONES>
+__device__ __forceinline__ void clear_lds(const Params& p, T* kl, T* vl) {
+    using D = Dims<KS>;
+    uint4* w = (uint4*)kl;
+    for (int i = threadIdx.x; i < (D::KELEMS + D::VELEMS) / 8; i += 256) w[i] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
+    if (ONES && threadIdx.x < 128) vl[threadIdx.x * D::VSTR + p.d] = __builtin_bit_cast(T, Ops<T>::kOne);
+    __syncthreads();
+}
+
+__device__ __forceinline__ long long out_row(const Params& p, int h, int r) {
+    const int tok = r / p.G, g = r - tok * p.G;
+    return (long long)tok * p.Hq + h * p.G + g;
+}
+
+// Least of x over the wave's lanes
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) x = min(x, __shfl_xor(x, off));
+    return __builtin_amdgcn_readfirstlane(x);
+}
+
+template <typename T, int KS, int QT, bool ONES>
+__device__ __forceinline__ void rows_way(const Params& p, const Item& it, char* lds) {
+    using D = Dims<KS>;
+    T* kl = (T*)lds;
+    T* vl = kl + D::KELEMS;
+    float* scales = (float*)(lds + D::kRowData);
+    int* flags = (int*)(scales + 128);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    Rows<T, KS, QT, ONES> R;
+    R.init(p, it.h, it.row_begin + wave * 32 * QT, it.row_end, lane, it.L);
+    int least = 0x7fffffff;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) least = min(least, R.lim[t]);
+    least = wave_min(least);                             // keys that all rows of the wave see
+    // the first row of the item sees least (rows in causal order): the workgroup's own bound without an exchange
+    const int block_least = p.causal ? min(it.L, max(0, it.L - p.n + 1 + (it.row_begin / p.G) % p.n)) : it.L;
+    const bool used = it.row_begin + wave * 32 * QT < it.row_end;
+    clear_lds<T, KS, ONES>(p, kl, vl);
+
+    Stager<T, KS, 256, 64> st;
+    auto load = [&](int v) {
+        const int seg = v >= it.TP;
+        st.load(p, seg, it.b, it.h, (seg ? v - it.TP : v) * 64, seg ? it.L : p.P, tid);
+    };
+    if (D::kAhead && it.v0 < it.v1) load(it.v0);
+    for (int v = it.v0; v < it.v1; ++v) {
+        const int buf = (v & 1) * 64, seg = v >= it.TP, key0 = (seg ? v - it.TP : v) * 64;
+        const bool edge = p.causal && seg && key0 + 64 > block_least;
+        if (edge) {
+            if (tid < 64) flags[buf + tid] = 0;
+            __syncthreads();
+        }
+        if (!D::kAhead) load(v);
+        st.store(p, kl + buf * D::KSTR, vl + buf * D::VSTR, scales + buf, edge, flags + buf, tid);
+        const bool scaled = st.fmt != SID_KV_NONE;
+        __syncthreads();                                 // also: every wave is done with the other buffer
+        if (D::kAhead && v + 1 < it.v1) load(v + 1);
+        if (used)
+#pragma unroll
+            for (int u = 0; u < 64; u += 32 * D::NS)
+                R.template tile<D::NS>(p, kl + (buf + u) * D::KSTR, vl + (buf + u) * D::VSTR, scales + buf + u, scaled, seg, key0 + u,
+                                       key0 + 64 > (seg ? least : p.P), edge, flags + buf + u, lane);
+    }
+
+    const int hi = lane >> 5;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int r = it.row_begin + wave * 32 * QT + t * 32 + (lane & 31);
+        const float sum = R.row_sum(p, t);
+        if (r >= it.row_end) continue;
+        const long long row = out_row(p, it.h, r);
+        if (p.part) {
+            const long long at = (long long)it.slot * p.B * p.n * p.Hq + row;
+            if (hi == 0) p.stats[at] = make_float2(R.reference(p, t), sum);
+            float* dst = p.part + at * p.d;
+#pragma unroll
+            for (int d = 0; d < D::DVB; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const int c = d * 32 + 2 * e + 4 * hi;
+                    if (c < p.d) *(float4*)(dst + c) = make_float4(R.o[t][d][e], R.o[t][d][e + 1], R.o[t][d][e + 2], R.o[t][d][e + 3]);
+                }
+        } else {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            char* dst = p.out + row * p.d * 2;
+#pragma unroll
+            for (int d = 0; d < D::DVB; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const int c = d * 32 + 2 * e + 4 * hi;
+                    if (c < p.d) store4<T>(dst + c * 2, R.o[t][d][e] * inv, R.o[t][d][e + 1] * inv, R.o[t][d][e + 2] * inv, R.o[t][d][e + 3] * inv);
+                }
+        }
+    }
+}
+
+// Orders one wave's LDS writes before its lanes' reads of one another's (the hardware keeps a wave's LDS operations in
+// order; this keeps the compiler from moving them).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <typename T, int KS, bool ONES>
+__device__ __forceinline__ void keys_way(const Params& p, const Item& it, char* lds) {
+    using D = Dims<KS>;
+    T* kl = (T*)lds;
+    T* vl = kl + D::KELEMS;
+    float* scales = (float*)(lds + D::kRowData);
+    int* flags = (int*)(scales + 128);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), buf = wave * 32;
+    Rows<T, KS, 1, ONES> R;
+    R.init(p, it.h, it.row_begin, it.row_end, lane, it.L);
+    const int least = wave_min(R.lim[0]);
+    clear_lds<T, KS, ONES>(p, kl, vl);
+
+    Stager<T, KS, 64, 32> st;
+    auto load = [&](int v) {
+        const int seg = v >= it.TP;
+        st.load(p, seg, it.b, it.h, (seg ? v - it.TP : v) * 32, seg ? it.L : p.P, lane);
+    };
+    if (D::kAhead && it.v0 + wave < it.v1) load(it.v0 + wave);
+    for (int v = it.v0 + wave; v < it.v1; v += 4) {
+        const int seg = v >= it.TP, key0 = (seg ? v - it.TP : v) * 32;
+        const bool edge = p.causal && seg && key0 + 32 > least;
+        wave_sync();                                     // the last tile's reads come before this one's writes
+        if (edge) {
+            if (lane < 32) flags[buf + lane] = 0;
+            wave_sync();
+        }
+        if (!D::kAhead) load(v);
+        st.store(p, kl + buf * D::KSTR, vl + buf * D::VSTR, scales + buf, edge, flags + buf, lane);
+        const bool scaled = st.fmt != SID_KV_NONE;
+        wave_sync();
+        if (D::kAhead && v + 4 < it.v1) load(v + 4);
+        R.template tile<1>(p, kl + buf * D::KSTR, vl + buf * D::VSTR, scales + buf, scaled, seg, key0, key0 + 32 > (seg ? least : p.P), edge, flags + buf, lane);
+    }
+
+    const float sum = R.row_sum(p, 0);
+    __syncthreads();
+    float* jo = (float*)lds;                             // [4][32][MSTR], then references and sums [4][32]
+    float* jm = jo + 4 * 32 * D::MSTR;
+    float* jl = jm + 128;
+    const int r32 = lane & 31, hi = lane >> 5;
+    if (hi == 0) { jm[buf + r32] = R.reference(p, 0); jl[buf + r32] = sum; }
+#pragma unroll
+    for (int d = 0; d < D::DVB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+            *(float4*)(jo + (buf + r32) * D::MSTR + d * 32 + 2 * e + 4 * hi) = make_float4(R.o[0][d][e], R.o[0][d][e + 1], R.o[0][d][e + 2], R.o[0][d][e + 3]);
+    __syncthreads();
+    const int rr = tid >> 3, r = it.row_begin + rr;      // 8 threads per row
+    if (r >= it.row_end) return;
+    float top = kNegInf, w[4], total = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = fmaxf(top, jm[k * 32 + rr]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        w[k] = jm[k * 32 + rr] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(jm[k * 32 + rr] - top);
+        total = __builtin_fmaf(w[k], jl[k * 32 + rr], total);
+    }
+    // a wave whose keys gave NaN has no finite reference but a NaN sum
+#pragma unroll
+    for (int k = 0; k < 4; ++k) if (!(jl[k * 32 + rr] == jl[k * 32 + rr])) total = __builtin_nanf("");
+    const long long row = out_row(p, it.h, r);
+    const long long at = (long long)it.slot * p.B * p.n * p.Hq + row;
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    if (p.part && (tid & 7) == 0) p.stats[at] = make_float2(top, total);
+    for (int c = (tid & 7) * 4; c < p.d; c += 32) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float4 o = *(const float4*)(jo + (k * 32 + rr) * D::MSTR + c);
+            a.x = __builtin_fmaf(w[k], o.x, a.x); a.y = __builtin_fmaf(w[k], o.y, a.y);
+            a.z = __builtin_fmaf(w[k], o.z, a.z); a.w = __builtin_fmaf(w[k], o.w, a.w);
+        }
+        if (p.part) *(float4*)(p.part + at * p.d + c) = a;
+        else store4<T>(p.out + (row * p.d + c) * 2, a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+    }
+}
+
+// QT > 1: items share rows only (many rows per image); QT == 1: either way, by the item's group.
+template <typename T, int KS, int QT, bool ONES>
+__global__ void __launch_bounds__(256, KS <= 8 ? 2 : 1) shared_kernel(Params p) {
+    extern __shared__ __align__(16) char lds[];
+    Item it;
+    bool by_keys;
+    if (!find_item(p, it, by_keys)) return;
+    if (QT == 1 && by_keys) keys_way<T, KS, ONES>(p, it, lds);
+    else rows_way<T, KS, QT, ONES>(p, it, lds);
+}
+
+template <typename T, int KS, int QT, bool ONES>
+int launch(const Params& p, unsigned grid, hipStream_t st) {
+    using D = Dims<KS>;
+    if (int rc = sid::allow_dynamic_lds<shared_kernel<T, KS, QT, ONES>>(D::kLds)) return rc;
+    hipLaunchKernelGGL((shared_kernel<T, KS, QT, ONES>), dim3(grid), dim3(256), D::kLds, st, p);
+    SID_CHECK_HIP(hipGetLastError());
+    return SID_OK;
+}
+
+// Classes of head_dim by KS; a head_dim that fills V's last block leaves no spare column for the row sum.
+constexpr int kClasses[6] = {3, 4, 5, 8, 10, 16};
+inline int class_of(int d) {
+    for (int ks : kClasses) if (d <= ks * 16) return ks;
+    return 0;
+}
+constexpr bool two_tiles(int ks) { return ks <= 4; }      // 64 rows per wave fit in the registers
+
+template <typename T>
+int launch_type(const Params& p, int qt, unsigned grid, hipStream_t st) {
+    const bool ones = p.d % 32 != 0 || p.d < 32 * ((class_of(p.d) + 1) / 2);
+    switch (class_of(p.d)) {
+        case 3: return qt == 2 ? launch<T, 3, 2, true>(p, grid, st) : launch<T, 3, 1, true>(p, grid, st);
+        case 4:
+            if (ones) return qt == 2 ? launch<T, 4, 2, true>(p, grid, st) : launch<T, 4, 1, true>(p, grid, st);
+            return qt == 2 ? launch<T, 4, 2, false>(p, grid, st) : launch<T, 4, 1, false>(p, grid, st);
+        case 5: return launch<T, 5, 1, true>(p, grid, st);
+        case 8: return ones ? launch<T, 8, 1, true>(p, grid, st) : launch<T, 8, 1, false>(p, grid, st);
+        case 10: return ones ? launch<T, 10, 1, true>(p, grid, st) : launch<T, 10, 1, false>(p, grid, st);
+        default: return ones ? launch<T, 16, 1, true>(p, grid, st) : launch<T, 16, 1, false>(p, grid, st);
+    }
+}
+
+int launch_bf16(const Params& p, int qt, unsigned grid, hipStream_t st);
+int launch_f16(const Params& p, int qt, unsigned grid, hipStream_t st);
+
+}  // namespace sid_shared

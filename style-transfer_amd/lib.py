@@ -10,13 +10,25 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SID_LIB_OVERRIDE") or os.path.join(HERE, "libsid.so")   # override: kernel experiments only
 
 SID_OK = 0
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 COMPUTE_BF16, COMPUTE_F32X3, COMPUTE_F16QK = 0, 1, 2
 LAYOUT_BHND, LAYOUT_BNHD = 0, 1
+ACT_NONE, ACT_SILU = 0, 1
+KV_NONE, KV_INT8, KV_E4M3 = 0, 1, 2
 STATIC_SCRATCH_BYTES = 64 << 20
 
 _c = ctypes
 _vp, _i, _f, _sz = _c.c_void_p, _c.c_int, _c.c_float, _c.c_size_t
+
+
+
+class KVSource(_c.Structure):
+    """sid_kv_source: keys and values of a prefix, or of the sequences' own part."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("k_stride", _c.c_longlong * 3),
+                ("v_stride", _c.c_longlong * 3), ("scale_stride", _c.c_longlong * 2), ("fmt", _i)]
+
+
+Strides = _c.c_longlong * 3
 
 # name -> (restype, argtypes): every symbol include/sid.h declares
 SIGNATURES = {
@@ -43,6 +55,13 @@ SIGNATURES = {
     "sid_hf_filter_radius": (_i, [_vp] * 4 + [_i] * 4 + [_i, _i, _vp]),
     "sid_residual_sum": (_i, [_vp] * 4 + [_c.c_longlong, _i, _vp]),
     "sid_masked_adain": (_i, [_vp] * 4 + [_i, _i, _vp] + [_i] * 5 + [_vp]),
+    "sid_kv_cache_write": (_i, [_vp] * 10 + [_i] * 7 + [_vp]),
+    "sid_kv_cache_read": (_i, [_vp] * 7 + [_i] * 7 + [_vp]),
+    "sid_shared_attn_workspace_bytes": (_sz, [_i] * 7),
+    "sid_shared_attn_fwd": (_i, [_vp] * 6 + [_i] * 7 + [_f] + [_i] * 2 + [_vp, _sz, _vp]),
+    "sid_group_norm_workspace_bytes": (_sz, [_i] * 6),
+    "sid_group_norm_act_fwd": (_i, [_vp] * 6 + [_i] * 4 + [_f] + [_i] * 2 + [_vp, _sz, _vp]),
+    "sid_group_norm_act_bwd": (_i, [_vp] * 9 + [_i] * 6 + [_vp, _sz, _vp]),
 }
 
 

@@ -424,3 +424,311 @@ def masked_adain(cnt, sty_char, sty_back=None, mask=None, out=None):
                                       mask.shape[0] if mask is not None else 0, mask.shape[1] if mask is not None else 0,
                                       out.data_ptr(), B, C, H, W, _dtype_code(cnt), _stream(dev)))
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# Key/value cache in 8 bits
+# ------------------------------------------------------------------------------------------------
+_DTYPES3 = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_KV_FORMATS = {torch.int8: _lib.KV_INT8, torch.float8_e4m3fn: _lib.KV_E4M3}
+
+
+def _need_device(dev, *ts):
+    """Every tensor in the memory of the one GPU `dev` (strides are the caller's matter)."""
+    if dev.type != "cuda":
+        raise RuntimeError("libsid kernels need tensors in GPU memory (got %s)" % dev)
+    for t in ts:
+        if t.device != dev:
+            raise RuntimeError("all tensors must be on the same device (%s and %s)" % (dev, t.device))
+
+
+def _rows16(t):
+    """`t` (..., d) with d contiguous and every row on a 16-byte boundary: itself, or a copy."""
+    es = t.element_size()
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s in st[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+class QuantKV:
+    """Keys and values of B sequences in 8 bits: codes (B, H, S, d) as torch.int8 or torch.float8_e4m3fn and one float32
+    scale per row (B, H, S); a code stands for code * scale.  Made empty by kv_cache(), filled by kv_cache_write(),
+    read by kv_cache_read() and, without becoming 16-bit tensors in memory first, by shared_prefix_attention()."""
+
+    def __init__(self, k_codes, k_scale, v_codes, v_scale):
+        if k_codes.dtype not in _KV_FORMATS or v_codes.dtype != k_codes.dtype:
+            raise TypeError("codes must be int8 or float8_e4m3fn, keys and values alike, got %s and %s" % (k_codes.dtype, v_codes.dtype))
+        if k_codes.dim() != 4 or v_codes.shape != k_codes.shape:
+            raise ValueError("codes must be two (B, H, S, d) tensors, got %s and %s" % (tuple(k_codes.shape), tuple(v_codes.shape)))
+        for s in (k_scale, v_scale):
+            if s.dtype != torch.float32 or s.shape != k_codes.shape[:3]:
+                raise ValueError("scales must be float32 (B, H, S) = %s, got %s %s" % (tuple(k_codes.shape[:3]), s.dtype, tuple(s.shape)))
+        for t in (k_codes, k_scale, v_codes, v_scale):
+            if not t.is_contiguous():
+                raise RuntimeError("tensors must be contiguous")
+            if t.device != k_codes.device:
+                raise RuntimeError("all tensors must be on the same device")
+        self.k_codes, self.k_scale, self.v_codes, self.v_scale = k_codes, k_scale, v_codes, v_scale
+        self.B, self.H, self.S, self.d = k_codes.shape
+        self.fmt = _KV_FORMATS[k_codes.dtype]
+
+    @property
+    def device(self):
+        return self.k_codes.device
+
+    def nbytes(self):
+        return 2 * (self.k_codes.numel() + 4 * self.k_scale.numel())
+
+    def _source(self):
+        H, S, d = self.H, self.S, self.d
+        st = _lib.Strides(H * S * d, S * d, d)
+        return _lib.KVSource(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                             st, st, (_lib._c.c_longlong * 2)(H * S, S), self.fmt)
+
+
+def kv_cache(batch, heads, length, head_dim, fmt="int8", device="cuda"):
+    """An empty QuantKV (every position reads as zeros): `length` positions for each of `batch` sequences.  fmt "int8"
+    (rows of even magnitude: half the error of e4m3 on normally distributed features) or "e4m3" (rows with a few
+    large values: the small ones keep their relative precision)."""
+    dt = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}.get(fmt)
+    if dt is None:
+        raise ValueError("cache format must be 'int8' or 'e4m3', got %r" % (fmt,))
+    if head_dim % 8 or not 8 <= head_dim <= 256:
+        raise ValueError("head_dim must be a multiple of 8 in [8, 256], got %d" % head_dim)
+    shape = (batch, heads, length, head_dim)
+    codes = [torch.zeros(shape, dtype=torch.uint8, device=device).view(dt) for _ in range(2)]
+    scales = [torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)]
+    return QuantKV(codes[0], scales[0], codes[1], scales[1])
+
+
+def _positions(start, B, dev):
+    if isinstance(start, int):
+        return torch.full((B,), start, dtype=torch.int32, device=dev)
+    if start.dtype != torch.int32 or tuple(start.shape) != (B,) or not start.is_contiguous():
+        raise ValueError("positions and lengths must be contiguous int32 (B,) = (%d,), got %s %s" % (B, start.dtype, tuple(start.shape)))
+    return start
+
+
+def kv_cache_write(cache, k, v, start=0, length=None):
+    """Quantise k, v (B, H, n, d) (float32, bfloat16 or float16; any strides with d contiguous) into positions start[b] + i of
+    sequence b.  start: an int, or an int32 (B,) tensor on the device (nothing is read back, so a decoding step can be
+    captured in a HIP graph).  length: int32 (B,) tensor, rows i >= length[b] are padding and not written; None: all n.
+    Positions outside the cache are skipped; everything else in it stays as it was.  One launch."""
+    L = _lib.load()
+    dev = cache.device
+    if k.shape != v.shape or k.dtype != v.dtype or k.dim() != 4:
+        raise ValueError("k and v must be two (B, H, n, d) tensors of one dtype")
+    B, H, n, d = k.shape
+    if (B, H, d) != (cache.B, cache.H, cache.d):
+        raise ValueError("the cache holds (B, H, d) = %s, the call has %s" % ((cache.B, cache.H, cache.d), (B, H, d)))
+    if k.dtype not in _DTYPES3:
+        raise TypeError("tensors must be float32, bfloat16 or float16, got %s" % k.dtype)
+    start = _positions(start, B, dev)
+    if length is not None:
+        length = _positions(length, B, dev)
+        _need_device(dev, length)
+    _need_device(dev, k, v, start)
+    k, v = _rows16(k), _rows16(v)
+    with torch.cuda.device(dev):
+        _lib.check(L.sid_kv_cache_write(k.data_ptr(), v.data_ptr(), _lib.Strides(*k.stride()[:3]), _lib.Strides(*v.stride()[:3]),
+                                        cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scale.data_ptr(),
+                                        cache.v_scale.data_ptr(), start.data_ptr(), None if length is None else length.data_ptr(),
+                                        B, H, n, cache.S, d, _DTYPES3[k.dtype], cache.fmt, _stream(dev)))
+
+
+def kv_cache_read(cache, start, n, dtype=torch.bfloat16):
+    """The n positions from start[b] on (int, or int32 (B,) tensor on the device) as numbers: k, v (B, H, n, d) in `dtype`.
+    Positions outside the cache give zeros.  One launch."""
+    L = _lib.load()
+    dev = cache.device
+    if dtype not in _DTYPES3:
+        raise TypeError("tensors must be float32, bfloat16 or float16, got %s" % dtype)
+    if n < 0:
+        raise ValueError("n must not be negative")
+    start = _positions(start, cache.B, dev)
+    _need_device(dev, start)
+    shape = (cache.B, cache.H, n, cache.d)
+    k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(L.sid_kv_cache_read(cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scale.data_ptr(),
+                                       cache.v_scale.data_ptr(), k.data_ptr(), v.data_ptr(), start.data_ptr(),
+                                       cache.B, cache.H, n, cache.S, cache.d, _DTYPES3[dtype], cache.fmt, _stream(dev)))
+    return k, v
+
+
+# ------------------------------------------------------------------------------------------------
+# Attention of a batch that shares a prefix
+# ------------------------------------------------------------------------------------------------
+def _pair_source(pair, shape, dtype, what):
+    """(k, v) tensors -> (KVSource, tensors to keep alive).  `shape`: (B, H, keys, d), or (H, keys, d) for a prefix."""
+    k, v = pair
+    for t in (k, v):
+        if t.shape != shape or t.dtype != dtype:
+            raise ValueError("%s: keys and values must be %s %s, got %s %s" % (what, tuple(shape), dtype, tuple(t.shape), t.dtype))
+    k, v = _rows16(k), _rows16(v)
+    ks, vs = k.stride()[:-1], v.stride()[:-1]
+    if len(shape) == 3:
+        ks, vs = (0,) + ks, (0,) + vs
+    return _lib.KVSource(k.data_ptr(), v.data_ptr(), None, None, _lib.Strides(*ks), _lib.Strides(*vs),
+                         (_lib._c.c_longlong * 2)(0, 0), _lib.KV_NONE), (k, v)
+
+
+def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False, scale=None, prefix_len=None, out=None):
+    """Attention of a batch whose sequences share a prefix of keys and values, under one softmax with their own keys.
+
+    q (B, Hq, n, d) bfloat16 or float16, any strides with d contiguous; n = 1 for a decoding step.
+    prefix: (k, v) of shape (Hkv, P, d), one copy for the whole batch, or a QuantKV with B = 1; None: no prefix.
+        prefix_len: only its first keys (an int); None: all.
+    own: (k, v) of shape (B, Hkv, S, d), or a QuantKV with the batch's B; None: none.
+        own_len: int32 (B,) tensor on the device, how many of its own keys each sequence has (clamped to [0, S]).
+        causal: query i of a sequence sees its own keys j <= own_len - n + i.
+    Hq must be a multiple of Hkv (query head h reads key/value head h // (Hq // Hkv)).  scale: d ** -0.5 if None.
+    -> (B, n, Hq*d) of q's dtype.  A query that sees no key gives zeros."""
+    L = _lib.load()
+    dev = q.device
+    if q.dim() != 4:
+        raise ValueError("q must be (B, Hq, n, d), got %s" % (tuple(q.shape),))
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("q must be bfloat16 or float16, got %s" % q.dtype)
+    B, Hq, n, d = q.shape
+    _need_device(dev)
+    Hkv, P, S, src, keep = None, 0, 0, [None, None], []
+    for i, (part, what) in enumerate(((prefix, "prefix"), (own, "own part"))):
+        if part is None:
+            continue
+        if isinstance(part, QuantKV):
+            if part.B != (B if i else 1) or part.d != d:
+                raise ValueError("%s: the cache holds (B, d) = %s, the call needs %s" % (what, (part.B, part.d), (B if i else 1, d)))
+            _need_device(dev, part.k_codes)
+            heads, keys = part.H, part.S
+            src[i] = part._source()
+        else:
+            k, v = part
+            if k.dim() != (4 if i else 3):
+                raise ValueError("%s: keys must be %s, got %s" % (what, "(B, H, S, d)" if i else "(H, P, d)", tuple(k.shape)))
+            _need_device(dev, k, v)
+            heads, keys = k.shape[-3], k.shape[-2]
+            src[i], alive = _pair_source(part, ((B,) if i else ()) + (heads, keys, d), q.dtype, what)
+            keep.append(alive)
+        if Hkv not in (None, heads):
+            raise ValueError("prefix and own part differ in heads: %d and %d" % (Hkv, heads))
+        Hkv = heads
+        if i:
+            S = keys
+        else:
+            P = keys
+    if Hkv is None:
+        raise ValueError("neither a prefix nor own keys")
+    if prefix_len is not None:
+        if not 0 <= prefix_len <= P:
+            raise ValueError("prefix_len %d is outside [0, %d]" % (prefix_len, P))
+        P = int(prefix_len)
+    if own_len is not None:
+        own_len = _positions(own_len, B, dev)
+        _need_device(dev, own_len)
+    q = _rows16(q)
+    if out is None:
+        out = torch.empty((B, n, Hq * d), dtype=q.dtype, device=dev)
+    elif out.shape != (B, n, Hq * d) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
+        raise ValueError("out must be a contiguous %s %s on %s" % ((B, n, Hq * d), q.dtype, dev))
+    nbytes = L.sid_shared_attn_workspace_bytes(B, Hq, Hkv, n, d, P, S)
+    if nbytes == 0:
+        raise _lib.SidError(-22, L.sid_last_error().decode())
+    ws = _workspace(dev, nbytes)
+    with torch.cuda.device(dev):
+        _lib.check(L.sid_shared_attn_fwd(
+            q.data_ptr(), _lib.Strides(*q.stride()[:3]), None if src[0] is None else _lib._c.addressof(src[0]),
+            None if src[1] is None else _lib._c.addressof(src[1]), None if own_len is None else own_len.data_ptr(),
+            out.data_ptr(), B, Hq, Hkv, n, d, P, S, float(d ** -0.5 if scale is None else scale), int(causal),
+            _DTYPES3[q.dtype], ws.data_ptr(), ws.numel(), _stream(dev)))
+    return out
+
+
+# ------------------------------------------------------------------------------------------------
+# Group normalisation with an activation, channels last
+# ------------------------------------------------------------------------------------------------
+_ACTS = {"none": _lib.ACT_NONE, "silu": _lib.ACT_SILU}
+
+
+def _norm_shape(x, groups):
+    """(B, N, C) of a channels-last tensor: (B, C, H, W) in channels-last memory, or (B, N, C) contiguous."""
+    if x.dim() == 4:
+        if not x.is_contiguous(memory_format=torch.channels_last):
+            raise ValueError("a (B, C, H, W) tensor must be in channels-last memory (x.contiguous(memory_format=torch.channels_last))")
+        B, C, H, W = x.shape
+        return B, H * W, C
+    if x.dim() == 3:
+        if not x.is_contiguous():
+            raise ValueError("a (B, N, C) tensor must be contiguous")
+        return tuple(x.shape)
+    raise ValueError("x must be (B, C, H, W) in channels-last memory or (B, N, C), got %s" % (tuple(x.shape),))
+
+
+def _norm_forward(x, groups, weight, bias, eps, act):
+    L = _lib.load()
+    dev = x.device
+    B, N, C = _norm_shape(x, groups)
+    if x.dtype not in _DTYPES3:
+        raise TypeError("x must be float32, bfloat16 or float16, got %s" % x.dtype)
+    for t in (weight, bias):
+        if t is not None and (t.shape != (C,) or t.dtype != torch.float32 or not t.is_contiguous()):
+            raise ValueError("weight and bias must be contiguous float32 (C,) = (%d,)" % C)
+    _need_device(dev, *[t for t in (weight, bias) if t is not None])
+    y = torch.empty_like(x)
+    stats = torch.empty((2, B, groups), dtype=torch.float32, device=dev)
+    nbytes = L.sid_group_norm_workspace_bytes(B, N, C, groups, _DTYPES3[x.dtype], 0)
+    if nbytes == 0:
+        raise _lib.SidError(-22, L.sid_last_error().decode())
+    ws = _workspace(dev, nbytes)
+    with torch.cuda.device(dev):
+        _lib.check(L.sid_group_norm_act_fwd(
+            x.data_ptr(), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
+            stats.data_ptr(), stats.data_ptr() + 4 * B * groups, B, N, C, groups, float(eps), _ACTS[act], _DTYPES3[x.dtype],
+            ws.data_ptr(), ws.numel(), _stream(dev)))
+    return y, stats
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        y, stats = _norm_forward(x, groups, weight, bias, eps, act)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.groups, ctx.act = groups, act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        L = _lib.load()
+        dev, G = x.device, ctx.groups
+        B, N, C = _norm_shape(x, G)
+        dy = dy.to(x.dtype).contiguous(memory_format=torch.channels_last if x.dim() == 4 else torch.contiguous_format)
+        dx = torch.empty_like(x)
+        dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
+        db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
+        ws = _workspace(dev, L.sid_group_norm_workspace_bytes(B, N, C, G, _DTYPES3[x.dtype], 1))
+        ptr = lambda t: None if t is None else t.data_ptr()
+        with torch.cuda.device(dev):
+            _lib.check(L.sid_group_norm_act_bwd(
+                dy.data_ptr(), x.data_ptr(), ptr(weight), ptr(bias), stats.data_ptr(), stats.data_ptr() + 4 * B * G, dx.data_ptr(),
+                ptr(dw), ptr(db), B, N, C, G, _ACTS[ctx.act], _DTYPES3[x.dtype], ws.data_ptr(), ws.numel(), _stream(dev)))
+        return dx, dw, db, None, None, None
+
+
+def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="silu"):
+    """act(group_norm(x) * weight + bias) over channels-last tensors, differentiable in x, weight and bias.
+
+    x (B, C, H, W) in channels-last memory, or tokens (B, N, C) contiguous; float32, bfloat16 or float16.  weight, bias:
+    float32 (C,) or None (other float types are cast, with gradients).  act: "silu" or "none".  Statistics, gradients of
+    weight and bias and all arithmetic are float32; y has x's dtype and memory order.  Needs at least one value."""
+    if act not in _ACTS:
+        raise ValueError("act must be 'silu' or 'none', got %r" % (act,))
+    if weight is not None and weight.dtype != torch.float32:
+        weight = weight.float()
+    if bias is not None and bias.dtype != torch.float32:
+        bias = bias.float()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _GroupNormAct.apply(x, weight, bias, groups, eps, act)
+    return _norm_forward(x, groups, weight, bias, eps, act)[0]
