@@ -6,31 +6,56 @@
 namespace sid_shared {
 namespace {
 
-// out = sum over slots of 2^(m - M) part / sum of 2^(m - M) l.  One thread per four columns of a row.
+constexpr int kMaxSlots = 128;
+
+// out = sum over slots of 2^(m - M) part / sum of 2^(m - M) l.  A thread owns four columns (quad) of one row and every
+// (1 << log_sg)-th slot; 2^log_q quads, so a row has 2^(log_q + log_sg) threads.  They read the row's references and sums
+// together, and what they gather from their slots is joined through LDS.
 template <typename T>
 __global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ part, const float2* __restrict__ stats, char* __restrict__ out,
-                                                      long long rows, int d, int slots) {
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int quads = d / 4;
-    const long long row = id / quads;
-    if (row >= rows) return;
-    const int c = (int)(id - row * quads) * 4;
+                                                      int rows, int d, int slots, int log_q, int log_sg) {
+    __shared__ float2 st[16 * kMaxSlots];            // (weight, sum) per row of the workgroup and slot
+    __shared__ float4 acc[256];
+    __shared__ float tot[256];
+    const int tid = threadIdx.x, per_row = 1 << (log_q + log_sg), lr = tid >> (log_q + log_sg);
+    const int in_row = tid & (per_row - 1), quad = in_row & ((1 << log_q) - 1), sg = in_row >> log_q;
+    const int row = blockIdx.x * (256 / per_row) + lr;
+    const bool live = row < rows;
+    float2* mine = st + lr * slots;
+    for (int s = in_row; s < slots; s += per_row) mine[s] = live ? stats[(long long)s * rows + row] : make_float2(kNegInf, 0.f);
+    __syncthreads();
     float top = kNegInf;
-    for (int s = 0; s < slots; ++s) top = fmaxf(top, stats[(long long)s * rows + row].x);
+    for (int s = 0; s < slots; ++s) top = fmaxf(top, mine[s].x);
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     float total = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < slots; ++s) {
-        const float2 st = stats[(long long)s * rows + row];
-        const float4 o = *(const float4*)(part + ((long long)s * rows + row) * d + c);
-        // an empty slot has reference -inf and sum 0; one whose keys gave NaN may have that reference and a NaN sum
-        const float w = st.x == kNegInf ? (st.y == 0.f ? 0.f : st.y) : __builtin_amdgcn_exp2f(st.x - top);
-        total = __builtin_fmaf(w, st.y, total);
-        a.x = __builtin_fmaf(w, o.x, a.x); a.y = __builtin_fmaf(w, o.y, a.y);
-        a.z = __builtin_fmaf(w, o.z, a.z); a.w = __builtin_fmaf(w, o.w, a.w);
+    if (live && quad * 4 < d) {
+        const float* src = part + (long long)row * d + quad * 4;
+#pragma unroll 8
+        for (int s = sg; s < slots; s += 1 << log_sg) {
+            const float2 v = mine[s];
+            const float4 o = *(const float4*)(src + (long long)s * rows * d);
+            // an empty slot has reference -inf and sum 0; one whose keys gave NaN may have that reference and a NaN sum
+            const float w = v.x == kNegInf ? (v.y == 0.f ? 0.f : v.y) : __builtin_amdgcn_exp2f(v.x - top);
+            total = __builtin_fmaf(w, v.y, total);
+            a.x = __builtin_fmaf(w, o.x, a.x); a.y = __builtin_fmaf(w, o.y, a.y);
+            a.z = __builtin_fmaf(w, o.z, a.z); a.w = __builtin_fmaf(w, o.w, a.w);
+        }
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    store4<T>(out + (row * d + c) * 2, a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+    for (int h = 1 << log_sg >> 1; h >= 1; h >>= 1) {
+        acc[tid] = a;
+        tot[tid] = total;
+        __syncthreads();
+        if (sg < h) {
+            const float4 o = acc[tid + (h << log_q)];
+            a.x += o.x; a.y += o.y; a.z += o.z; a.w += o.w;
+            total += tot[tid + (h << log_q)];
+        }
+        __syncthreads();
+    }
+    if (sg == 0 && live && quad * 4 < d) {
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        store4<T>(out + ((long long)row * d + quad * 4) * 2, a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+    }
 }
 
 struct Plan {
@@ -45,11 +70,11 @@ constexpr int kFill = 512;          // workgroups that fill the chip: two on eac
 int padded(int items) { return (items + kXcd - 1) / kXcd * kXcd; }
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// Splits of a key range of `keys` so that `items` x splits workgroups fill the chip, each with at least `least` keys.
-int splits_for(long long items, long long keys, int least) {
-    long long s = (kFill + items - 1) / items;
+// Splits of a key range of `keys` into at most `fill` workgroups over `items`, each with at least `least` keys.
+int splits_for(long long items, long long keys, long long fill, int least) {
+    long long s = fill / items;
     if (s > keys / least) s = keys / least;
-    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+    return (int)(s < 1 ? 1 : s > kMaxSlots / 2 ? kMaxSlots / 2 : s);
 }
 
 Plan make_plan(int B, int Hkv, int G, int n, int d, int P, int S) {
@@ -64,19 +89,17 @@ Plan make_plan(int B, int Hkv, int G, int n, int d, int P, int S) {
         // many rows per image: each tile walks prefix and own keys
         pl.qt = two_tiles(class_of(d)) && rows > 128 ? 2 : 1;
         const int tile = 128 * pl.qt, tiles = ceil_div(rows, tile);
-        add(0, tiles, tile, splits_for((long long)B * Hkv * tiles, (long long)P + S, 512), 1, 0, (P ? 1 : 0) | (S ? 2 : 0));
+        const long long items = (long long)B * Hkv * tiles;
+        add(0, tiles, tile, splits_for(items, (long long)P + S, kFill + items / 2, 512), 1, 0, (P ? 1 : 0) | (S ? 2 : 0));
     } else {
+        // the chip's workgroups are shared out by the keys that prefix and own parts have to walk
+        const long long all = rows * B;
+        const int by_keys = all <= 32, ptile = by_keys ? 32 : 128, ptiles = ceil_div(all, ptile), otiles = ceil_div(rows, 32);
+        const long long pitems = (long long)Hkv * ptiles, oitems = (long long)B * Hkv * otiles, pwork = pitems * P, owork = oitems * S;
         int k = 0;
-        if (P) {
-            const long long all = rows * B;
-            const int by_keys = all <= 32, tile = by_keys ? 32 : 128, tiles = ceil_div(all, tile);
-            add(k++, tiles, tile, splits_for((long long)Hkv * tiles, P, 256), 0, by_keys, 1);
-        }
-        if (S) {
-            const int tiles = ceil_div(rows, 32);
-            add(k++, tiles, 32, splits_for((long long)B * Hkv * tiles, S, 256), 1, 1, 2);
-        }
-        if (!k) add(0, ceil_div(rows, 32), 32, 1, 1, 1, 0);          // no keys at all: zeros
+        if (P) add(k++, ptiles, ptile, splits_for(pitems, P, kFill * pwork / (pwork + owork) + pitems / 2, by_keys ? 128 : 256), 0, by_keys, 1);
+        if (S) add(k++, otiles, 32, splits_for(oitems, S, kFill * owork / (pwork + owork) + oitems / 2, 128), 1, 1, 2);
+        if (!k) add(0, otiles, 32, 1, 1, 1, 0);          // no keys at all: zeros
     }
     pl.blocks0 = padded(pl.g[0].items);
     pl.grid = (unsigned)(pl.blocks0 + padded(pl.g[1].items));
@@ -165,9 +188,14 @@ extern "C" int sid_shared_attn_fwd(const void* q, const long long* q_stride, con
     const hipStream_t st = (hipStream_t)stream;
     if (int rc = dtype == SID_DTYPE_BF16 ? launch_bf16(p, pl.qt, pl.grid, st) : launch_f16(p, pl.qt, pl.grid, st)) return rc;
     if (need) {
-        const unsigned grid = (unsigned)((rows * (d / 4) + 255) / 256);
-        if (dtype == SID_DTYPE_BF16) hipLaunchKernelGGL(combine_kernel<__bf16>, dim3(grid), dim3(256), 0, st, p.part, p.stats, p.out, rows, d, pl.slots);
-        else hipLaunchKernelGGL(combine_kernel<_Float16>, dim3(grid), dim3(256), 0, st, p.part, p.stats, p.out, rows, d, pl.slots);
+        // quads of a row to a power of two; slots shared by up to eight threads while that leaves each one a few
+        int log_q = 4, log_sg = 0;
+        while ((4 << log_q) < d) ++log_q;
+        while (log_sg < 8 - log_q && (4 << log_sg) < pl.slots) ++log_sg;
+        const int per_block = 256 >> (log_q + log_sg);
+        const unsigned grid = (unsigned)((rows + per_block - 1) / per_block);
+        if (dtype == SID_DTYPE_BF16) hipLaunchKernelGGL(combine_kernel<__bf16>, dim3(grid), dim3(256), 0, st, p.part, p.stats, p.out, (int)rows, d, pl.slots, log_q, log_sg);
+        else hipLaunchKernelGGL(combine_kernel<_Float16>, dim3(grid), dim3(256), 0, st, p.part, p.stats, p.out, (int)rows, d, pl.slots, log_q, log_sg);
         SID_CHECK_HIP(hipGetLastError());
     }
     return SID_OK;

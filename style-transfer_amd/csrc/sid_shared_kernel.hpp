@@ -30,6 +30,7 @@
 #include "sid_common.h"
 
 #include <cstdint>
+#include <type_traits>
 
 namespace sid_shared {
 
@@ -41,6 +42,7 @@ typedef __attribute__((ext_vector_type(8))) short s16x8;
 
 constexpr int kXcd = 8;
 constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kNone = -3e38f;       // softmax reference before the first key: finite, so that no difference is NaN
 
 struct Source {                      // keys and values of the prefix, or of the images' own part
     const char *k, *v;
@@ -87,7 +89,11 @@ template <> struct Ops<_Float16> {
     static __device__ __forceinline__ f32x16 mfma(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+// x of the lane's own half and of lane ^ 32: (lower half's, upper half's) in every lane
+__device__ __forceinline__ float2 both_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
 // The head-dim classes: KS steps of 16 in q.k, DVB blocks of 32 in V, LPR lanes that stage one row (8 elements each).
 template <int KS> struct Dims {
@@ -104,45 +110,64 @@ template <int KS> struct Dims {
     static constexpr bool kAhead = KS <= 10;         // a tile waits in registers while the one before it is computed
 };
 
+// Keys and values of one (image, head) of a part, as a loop over its tiles reads them.
+struct Stream {
+    const char *k, *v;
+    const float *ks, *vs;
+    int kn, vn, fmt, end;            // keys from `end` on are not there
+
+    __device__ __forceinline__ Stream(const Params& p, int seg, int b, int h, int keys) {
+        const Source& s = p.src[seg];
+        const int bi = seg ? b : 0;
+        k = s.k + bi * s.kb + h * s.kh;
+        v = s.v + bi * s.vb + h * s.vh;
+        ks = s.ks + bi * s.sb + h * s.sh;
+        vs = s.vs + bi * s.sb + h * s.sh;
+        kn = s.kn; vn = s.vn; fmt = s.fmt; end = keys;
+    }
+};
+
 // One key tile on its way from memory to LDS.  NT threads, KT keys.
 template <typename T, int KS, int NT, int KT>
 struct Stager {
     using D = Dims<KS>;
     static constexpr int RPP = NT / D::LPR, NJ = KT / RPP;
     uint4 k[NJ], v[NJ];
-    int fmt;
 
-    __device__ __forceinline__ void load(const Params& p, int seg, int b, int h, int key0, int end, int t) {
-        const Source& s = p.src[seg];
-        fmt = s.fmt;
+    // whole: the tile ends before s.end.
+    __device__ __forceinline__ void load(const Params& p, const Stream& s, int key0, bool whole, int t) {
         const int col = t % D::LPR, row = t / D::LPR;
-        const bool live = col * 8 < p.d;
-        const int bi = seg ? b : 0;
-        const int step = s.fmt == SID_KV_NONE ? 16 : 8;
-        const char* kp = s.k + bi * s.kb + h * s.kh + (long long)key0 * s.kn;
-        const char* vp = s.v + bi * s.vb + h * s.vh + (long long)key0 * s.vn;
+        if (col * 8 >= p.d) return;                      // lanes behind head_dim have nothing to load or to store
+        const char* kp = s.k + (long long)key0 * s.kn;
+        const char* vp = s.v + (long long)key0 * s.vn;
         if (s.fmt == SID_KV_NONE) {
+            const unsigned ko = row * s.kn + col * 16, vo = row * s.vn + col * 16;
+            if (whole) {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int r = row + j * RPP;
-                k[j] = v[j] = make_uint4(0u, 0u, 0u, 0u);
-                if (live && key0 + r < end) {
-                    k[j] = *(const uint4*)(kp + (unsigned)(r * s.kn + col * step));
-                    v[j] = *(const uint4*)(vp + (unsigned)(r * s.vn + col * step));
+                for (int j = 0; j < NJ; ++j) {
+                    k[j] = *(const uint4*)(kp + j * RPP * s.kn + ko);
+                    v[j] = *(const uint4*)(vp + j * RPP * s.vn + vo);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    k[j] = v[j] = make_uint4(0u, 0u, 0u, 0u);
+                    if (key0 + row + j * RPP < s.end) {
+                        k[j] = *(const uint4*)(kp + j * RPP * s.kn + ko);
+                        v[j] = *(const uint4*)(vp + j * RPP * s.vn + vo);
+                    }
                 }
             }
         } else {
-            const float* ks = s.ks + bi * s.sb + h * s.sh + key0;
-            const float* vs = s.vs + bi * s.sb + h * s.sh + key0;
+            const unsigned ko = row * s.kn + col * 8, vo = row * s.vn + col * 8;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                const int r = row + j * RPP;
-                k[j] = v[j] = make_uint4(0u, 0u, 0u, 0u);
-                if (live && key0 + r < end) {
-                    const uint2 a = *(const uint2*)(kp + (unsigned)(r * s.kn + col * step));
-                    const uint2 c = *(const uint2*)(vp + (unsigned)(r * s.vn + col * step));
-                    k[j] = make_uint4(a.x, a.y, __float_as_uint(ks[r]), 0u);
-                    v[j] = make_uint4(c.x, c.y, __float_as_uint(vs[r]), 0u);
+                const int r = key0 + row + j * RPP;
+                if (!whole) k[j] = v[j] = make_uint4(0u, 0u, 0u, 0u);
+                if (whole || r < s.end) {
+                    const uint2 a = *(const uint2*)(kp + j * RPP * s.kn + ko), c = *(const uint2*)(vp + j * RPP * s.vn + vo);
+                    k[j] = make_uint4(a.x, a.y, __float_as_uint(s.ks[r]), 0u);
+                    v[j] = make_uint4(c.x, c.y, __float_as_uint(s.vs[r]), 0u);
                 }
             }
         }
@@ -170,7 +195,7 @@ struct Stager {
 
     // `edge`: keys that some rows of the tile do not see are in it.  Their probability is zero, but zero times an
     // infinity or a NaN is not: such values become zeros and the key is flagged (rows that do see it turn NaN).
-    __device__ __forceinline__ void store(const Params& p, T* kl, T* vl, float* scale, bool edge, int* bad, int t) {
+    __device__ __forceinline__ void store(const Params& p, int fmt, T* kl, T* vl, float* scale, bool edge, int* bad, int t) {
         const int col = t % D::LPR, row = t / D::LPR;
         if (col * 8 >= p.d) return;
 #pragma unroll
@@ -224,7 +249,7 @@ struct Rows {
                 q[t][kk] = in && e < p.d ? *(const V8*)(src + e * 2) : V8{};
             }
             lim[t] = !in ? 0x7fffffff : p.causal ? min(L, max(0, L - p.n + 1 + i)) : L;
-            m[t] = kNegInf;
+            m[t] = kNone;
             l[t] = 0.f;
 #pragma unroll
             for (int d = 0; d < D::DVB; ++d)
@@ -233,11 +258,11 @@ struct Rows {
         }
     }
 
-    // NS sub-tiles of 32 keys in LDS; `scaled`: every key's logits carry its own factor; `masked`: some row sees only the keys
+    // NS sub-tiles of 32 keys in LDS.  codes: every key's logits carry its own factor.  masked: some row sees only the keys
     // below its own part's limit (seg), or below P.
     template <int NS>
-    __device__ __forceinline__ void tile(const Params& p, const T* kl, const T* vl, const float* scale, bool scaled, int seg, int key0, bool masked, bool edge,
-                                         const int* bad, int lane) {
+    __device__ __forceinline__ void tile(const Params& p, const T* kl, const T* vl, const float* scale, bool codes, int seg, int key0,
+                                         bool masked, bool edge, const int* bad, int lane) {
         const int r32 = lane & 31, hi = lane >> 5;
         f32x16 s[QT][NS];
 #pragma unroll
@@ -253,8 +278,8 @@ struct Rows {
                 for (int t = 0; t < QT; ++t) s[t][u] = Ops<T>::mfma(a, q[t][kk], s[t][u]);
             }
         }
-        const float c = scaled ? 1.f : p.c;
-        if (scaled) {
+        const float c = codes ? 1.f : p.c;
+        if (codes) {
 #pragma unroll
             for (int u = 0; u < NS; ++u)
 #pragma unroll
@@ -286,12 +311,13 @@ struct Rows {
             for (int u = 0; u < NS; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[t][u][e]);
-            mt = fmaxf(mt, other_half(mt)) * c;
+            const float2 halves = both_halves(mt);
+            mt = fmaxf(halves.x, halves.y) * c;
             // the reference moves only when a logit exceeds it by 2^8: probabilities stay below that, nothing overflows
-            const bool up = mt - m[t] > 8.f || (m[t] == kNegInf && mt > kNegInf);
+            const bool up = mt - m[t] > 8.f;
             if (__any(up)) {
                 const float mn = up ? mt : m[t];
-                const float alpha = m[t] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[t] - mn);
+                const float alpha = __builtin_amdgcn_exp2f(m[t] - mn);
                 m[t] = mn;
                 l[t] *= alpha;
 #pragma unroll
@@ -299,7 +325,7 @@ struct Rows {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[t][d][e] *= alpha;
             }
-            const float off = m[t] == kNegInf ? 0.f : Ops<T>::kBias - m[t];
+            const float off = Ops<T>::kBias - m[t];
 #pragma unroll
             for (int u = 0; u < NS; ++u) {
 #pragma unroll
@@ -338,12 +364,12 @@ struct Rows {
             for (int d = 0; d < D::DVB; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) sum = d * 32 + 2 * e == p.d ? o[t][d][e] : sum;
-            const float low = other_half(sum);
-            return (threadIdx.x & 32) ? low : sum;
+            return both_halves(sum).x;
         }
-        return sum + other_half(sum);
+        const float2 halves = both_halves(sum);
+        return halves.x + halves.y;
     }
-    __device__ __forceinline__ float reference(const Params& p, int t) const { return m[t] == kNegInf ? kNegInf : m[t] - Ops<T>::kBias; }
+    __device__ __forceinline__ float reference(const Params& p, int t) const { return m[t] == kNone ? kNegInf : m[t] - Ops<T>::kBias; }
 };
 
 template <typename T>
@@ -407,13 +433,6 @@ __device__ __forceinline__ long long out_row(const Params& p, int h, int r) {
     return (long long)tok * p.Hq + h * p.G + g;
 }
 
-// Least of x over the wave's lanes
-__device__ __forceinline__ int wave_min(int x) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) x = min(x, __shfl_xor(x, off));
-    return __builtin_amdgcn_readfirstlane(x);
-}
-
 template <typename T, int KS, int QT, bool ONES>
 __device__ __forceinline__ void rows_way(const Params& p, const Item& it, char* lds) {
     using D = Dims<KS>;
@@ -424,38 +443,35 @@ __device__ __forceinline__ void rows_way(const Params& p, const Item& it, char* 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     Rows<T, KS, QT, ONES> R;
     R.init(p, it.h, it.row_begin + wave * 32 * QT, it.row_end, lane, it.L);
-    int least = 0x7fffffff;
-#pragma unroll
-    for (int t = 0; t < QT; ++t) least = min(least, R.lim[t]);
-    least = wave_min(least);                             // keys that all rows of the wave see
-    // the first row of the item sees least (rows in causal order): the workgroup's own bound without an exchange
-    const int block_least = p.causal ? min(it.L, max(0, it.L - p.n + 1 + (it.row_begin / p.G) % p.n)) : it.L;
-    const bool used = it.row_begin + wave * 32 * QT < it.row_end;
+    // own keys that every row of the item sees: the first row's (in causal order rows see ever more)
+    const int least = p.causal ? min(it.L, max(0, it.L - p.n + 1 + (it.row_begin / p.G) % p.n)) : it.L;
     clear_lds<T, KS, ONES>(p, kl, vl);
 
     Stager<T, KS, 256, 64> st;
-    auto load = [&](int v) {
-        const int seg = v >= it.TP;
-        st.load(p, seg, it.b, it.h, (seg ? v - it.TP : v) * 64, seg ? it.L : p.P, tid);
-    };
-    if (D::kAhead && it.v0 < it.v1) load(it.v0);
-    for (int v = it.v0; v < it.v1; ++v) {
-        const int buf = (v & 1) * 64, seg = v >= it.TP, key0 = (seg ? v - it.TP : v) * 64;
-        const bool edge = p.causal && seg && key0 + 64 > block_least;
-        if (edge) {
-            if (tid < 64) flags[buf + tid] = 0;
-            __syncthreads();
-        }
-        if (!D::kAhead) load(v);
-        st.store(p, kl + buf * D::KSTR, vl + buf * D::VSTR, scales + buf, edge, flags + buf, tid);
-        const bool scaled = st.fmt != SID_KV_NONE;
-        __syncthreads();                                 // also: every wave is done with the other buffer
-        if (D::kAhead && v + 1 < it.v1) load(v + 1);
-        if (used)
+    int buf = 0;
+    for (int seg = 0; seg < 2; ++seg) {
+        const int t0 = seg ? max(it.v0 - it.TP, 0) : it.v0, t1 = seg ? it.v1 - it.TP : min(it.v1, it.TP);
+        if (t0 >= t1) continue;
+        const Stream s(p, seg, it.b, it.h, seg ? it.L : p.P);
+        const int seen = seg ? least : p.P;              // tiles that end before it need no mask
+        if (D::kAhead) st.load(p, s, t0 * 64, t0 * 64 + 64 <= s.end, tid);
+        for (int t = t0; t < t1; ++t) {
+            const int key0 = t * 64;
+            const bool masked = key0 + 64 > seen, edge = masked && p.causal && seg;
+            if (edge) {
+                if (tid < 64) flags[buf + tid] = 0;
+                __syncthreads();
+            }
+            if (!D::kAhead) st.load(p, s, key0, key0 + 64 <= s.end, tid);
+            st.store(p, s.fmt, kl + buf * D::KSTR, vl + buf * D::VSTR, scales + buf, edge, flags + buf, tid);
+            __syncthreads();                             // also: every wave is done with the other buffer
+            if (D::kAhead && t + 1 < t1) st.load(p, s, key0 + 64, key0 + 128 <= s.end, tid);
 #pragma unroll
             for (int u = 0; u < 64; u += 32 * D::NS)
-                R.template tile<D::NS>(p, kl + (buf + u) * D::KSTR, vl + (buf + u) * D::VSTR, scales + buf + u, scaled, seg, key0 + u,
-                                       key0 + 64 > (seg ? least : p.P), edge, flags + buf + u, lane);
+                R.template tile<D::NS>(p, kl + (buf + u) * D::KSTR, vl + (buf + u) * D::VSTR, scales + buf + u, s.fmt != SID_KV_NONE, seg, key0 + u,
+                                       masked, edge, flags + buf + u, lane);
+            buf ^= 64;
+        }
     }
 
     const int hi = lane >> 5;
@@ -507,29 +523,31 @@ __device__ __forceinline__ void keys_way(const Params& p, const Item& it, char* 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), buf = wave * 32;
     Rows<T, KS, 1, ONES> R;
     R.init(p, it.h, it.row_begin, it.row_end, lane, it.L);
-    const int least = wave_min(R.lim[0]);
+    const int least = p.causal ? min(it.L, max(0, it.L - p.n + 1 + (it.row_begin / p.G) % p.n)) : it.L;
     clear_lds<T, KS, ONES>(p, kl, vl);
 
     Stager<T, KS, 64, 32> st;
-    auto load = [&](int v) {
-        const int seg = v >= it.TP;
-        st.load(p, seg, it.b, it.h, (seg ? v - it.TP : v) * 32, seg ? it.L : p.P, lane);
-    };
-    if (D::kAhead && it.v0 + wave < it.v1) load(it.v0 + wave);
-    for (int v = it.v0 + wave; v < it.v1; v += 4) {
-        const int seg = v >= it.TP, key0 = (seg ? v - it.TP : v) * 32;
-        const bool edge = p.causal && seg && key0 + 32 > least;
-        wave_sync();                                     // the last tile's reads come before this one's writes
-        if (edge) {
-            if (lane < 32) flags[buf + lane] = 0;
+    for (int seg = 0; seg < 2; ++seg) {
+        const int t0 = (seg ? max(it.v0 - it.TP, 0) : it.v0) + wave, t1 = seg ? it.v1 - it.TP : min(it.v1, it.TP);
+        if (t0 >= t1) continue;
+        const Stream s(p, seg, it.b, it.h, seg ? it.L : p.P);
+        const int seen = seg ? least : p.P;
+        if (D::kAhead) st.load(p, s, t0 * 32, t0 * 32 + 32 <= s.end, lane);
+        for (int t = t0; t < t1; t += 4) {
+            const int key0 = t * 32;
+            const bool masked = key0 + 32 > seen, edge = masked && p.causal && seg;
+            wave_sync();                                 // the last tile's reads come before this one's writes
+            if (edge) {
+                if (lane < 32) flags[buf + lane] = 0;
+                wave_sync();
+            }
+            if (!D::kAhead) st.load(p, s, key0, key0 + 32 <= s.end, lane);
+            st.store(p, s.fmt, kl + buf * D::KSTR, vl + buf * D::VSTR, scales + buf, edge, flags + buf, lane);
             wave_sync();
+            if (D::kAhead && t + 4 < t1) st.load(p, s, key0 + 128, key0 + 160 <= s.end, lane);
+            R.template tile<1>(p, kl + buf * D::KSTR, vl + buf * D::VSTR, scales + buf, s.fmt != SID_KV_NONE, seg, key0, masked, edge,
+                               flags + buf, lane);
         }
-        if (!D::kAhead) load(v);
-        st.store(p, kl + buf * D::KSTR, vl + buf * D::VSTR, scales + buf, edge, flags + buf, lane);
-        const bool scaled = st.fmt != SID_KV_NONE;
-        wave_sync();
-        if (D::kAhead && v + 4 < it.v1) load(v + 4);
-        R.template tile<1>(p, kl + buf * D::KSTR, vl + buf * D::VSTR, scales + buf, scaled, seg, key0, key0 + 32 > (seg ? least : p.P), edge, flags + buf, lane);
     }
 
     const float sum = R.row_sum(p, 0);

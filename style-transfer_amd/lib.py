@@ -5,6 +5,7 @@ or an entry point fails, the caller gets an exception that says so.
 """
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SID_LIB_OVERRIDE") or os.path.join(HERE, "libsid.so")   # override: kernel experiments only
@@ -22,13 +23,10 @@ _vp, _i, _f, _sz = _c.c_void_p, _c.c_int, _c.c_float, _c.c_size_t
 
 
 
-class KVSource(_c.Structure):
-    """sid_kv_source: keys and values of a prefix, or of the sequences' own part."""
-    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("k_stride", _c.c_longlong * 3),
-                ("v_stride", _c.c_longlong * 3), ("scale_stride", _c.c_longlong * 2), ("fmt", _i)]
-
-
-Strides = _c.c_longlong * 3
+# sid_kv_source as bytes (a call reads it before it returns): k, v, k_scale, v_scale, k_stride[3], v_stride[3],
+# scale_stride[2], fmt.  A packed bytes object costs a fifth of filling a ctypes structure.
+kv_source = struct.Struct("4P8qi4x").pack
+strides3 = struct.Struct("3q").pack
 
 # name -> (restype, argtypes): every symbol include/sid.h declares
 SIGNATURES = {

@@ -8,6 +8,8 @@ the other two.  The long-sequence kernels refuse "f16" for logit scales outside 
 PyTorch is used for device memory and streams only; all arithmetic of the path happens in
 libsid.so.  Every function raises if the library is missing or rejects the call.
 """
+import contextlib
+import functools
 import threading
 
 import torch
@@ -44,7 +46,15 @@ def _compute_code(compute):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)       # what current_stream(device).cuda_stream reads, 2 us sooner
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """The device context of a launch: nothing to switch (and 1.4 us less) when `device` is the current one."""
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 _retired = []        # superseded workspaces stay alive: a captured HIP graph may hold their address
@@ -444,11 +454,24 @@ def _need_device(dev, *ts):
 
 def _rows16(t):
     """`t` (..., d) with d contiguous and every row on a 16-byte boundary: itself, or a copy."""
-    es = t.element_size()
+    bits = t.data_ptr()
     st = t.stride()
-    if st[-1] == 1 and t.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s in st[:-1]):
+    es = t.element_size()
+    for s in st[:-1]:
+        bits |= s * es
+    if st[-1] == 1 and not bits & 15:
         return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(name, *shape):
+    """What a call of this shape needs, from the library (which refuses the shape with 0)."""
+    L = _lib.load()
+    n = getattr(L, name)(*shape)
+    if n == 0:
+        raise _lib.SidError(-22, L.sid_last_error().decode())
+    return n
 
 
 class QuantKV:
@@ -457,34 +480,29 @@ class QuantKV:
     read by kv_cache_read() and, without becoming 16-bit tensors in memory first, by shared_prefix_attention()."""
 
     def __init__(self, k_codes, k_scale, v_codes, v_scale):
-        if k_codes.dtype not in _KV_FORMATS or v_codes.dtype != k_codes.dtype:
+        fmt, shape, dev = _KV_FORMATS.get(k_codes.dtype), k_codes.shape, k_codes.device
+        if fmt is None or v_codes.dtype != k_codes.dtype:
             raise TypeError("codes must be int8 or float8_e4m3fn, keys and values alike, got %s and %s" % (k_codes.dtype, v_codes.dtype))
-        if k_codes.dim() != 4 or v_codes.shape != k_codes.shape:
-            raise ValueError("codes must be two (B, H, S, d) tensors, got %s and %s" % (tuple(k_codes.shape), tuple(v_codes.shape)))
-        for s in (k_scale, v_scale):
-            if s.dtype != torch.float32 or s.shape != k_codes.shape[:3]:
-                raise ValueError("scales must be float32 (B, H, S) = %s, got %s %s" % (tuple(k_codes.shape[:3]), s.dtype, tuple(s.shape)))
-        for t in (k_codes, k_scale, v_codes, v_scale):
-            if not t.is_contiguous():
-                raise RuntimeError("tensors must be contiguous")
-            if t.device != k_codes.device:
-                raise RuntimeError("all tensors must be on the same device")
+        if len(shape) != 4 or v_codes.shape != shape:
+            raise ValueError("codes must be two (B, H, S, d) tensors, got %s and %s" % (tuple(shape), tuple(v_codes.shape)))
+        if not k_scale.dtype == v_scale.dtype == torch.float32 or not k_scale.shape == v_scale.shape == shape[:3]:
+            raise ValueError("scales must be float32 (B, H, S) = %s" % (tuple(shape[:3]),))
+        if not (k_codes.is_contiguous() and v_codes.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+            raise RuntimeError("tensors must be contiguous")
+        if not v_codes.device == k_scale.device == v_scale.device == dev:
+            raise RuntimeError("all tensors must be on the same device")
         self.k_codes, self.k_scale, self.v_codes, self.v_scale = k_codes, k_scale, v_codes, v_scale
-        self.B, self.H, self.S, self.d = k_codes.shape
-        self.fmt = _KV_FORMATS[k_codes.dtype]
-
-    @property
-    def device(self):
-        return self.k_codes.device
+        self.B, self.H, self.S, self.d = shape
+        self.device, self.fmt = dev, fmt
 
     def nbytes(self):
         return 2 * (self.k_codes.numel() + 4 * self.k_scale.numel())
 
     def _source(self):
-        H, S, d = self.H, self.S, self.d
-        st = _lib.Strides(H * S * d, S * d, d)
-        return _lib.KVSource(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
-                             st, st, (_lib._c.c_longlong * 2)(H * S, S), self.fmt)
+        d, S = self.d, self.S
+        Sd, HS = S * d, self.H * S
+        return _lib.kv_source(self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                              HS * d, Sd, d, HS * d, Sd, d, HS, S, self.fmt)
 
 
 def kv_cache(batch, heads, length, head_dim, fmt="int8", device="cuda"):
@@ -530,8 +548,8 @@ def kv_cache_write(cache, k, v, start=0, length=None):
         _need_device(dev, length)
     _need_device(dev, k, v, start)
     k, v = _rows16(k), _rows16(v)
-    with torch.cuda.device(dev):
-        _lib.check(L.sid_kv_cache_write(k.data_ptr(), v.data_ptr(), _lib.Strides(*k.stride()[:3]), _lib.Strides(*v.stride()[:3]),
+    with _on(dev):
+        _lib.check(L.sid_kv_cache_write(k.data_ptr(), v.data_ptr(), _lib.strides3(*k.stride()[:3]), _lib.strides3(*v.stride()[:3]),
                                         cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scale.data_ptr(),
                                         cache.v_scale.data_ptr(), start.data_ptr(), None if length is None else length.data_ptr(),
                                         B, H, n, cache.S, d, _DTYPES3[k.dtype], cache.fmt, _stream(dev)))
@@ -550,7 +568,7 @@ def kv_cache_read(cache, start, n, dtype=torch.bfloat16):
     _need_device(dev, start)
     shape = (cache.B, cache.H, n, cache.d)
     k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.check(L.sid_kv_cache_read(cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scale.data_ptr(),
                                        cache.v_scale.data_ptr(), k.data_ptr(), v.data_ptr(), start.data_ptr(),
                                        cache.B, cache.H, n, cache.S, cache.d, _DTYPES3[dtype], cache.fmt, _stream(dev)))
@@ -560,18 +578,16 @@ def kv_cache_read(cache, start, n, dtype=torch.bfloat16):
 # ------------------------------------------------------------------------------------------------
 # Attention of a batch that shares a prefix
 # ------------------------------------------------------------------------------------------------
-def _pair_source(pair, shape, dtype, what):
-    """(k, v) tensors -> (KVSource, tensors to keep alive).  `shape`: (B, H, keys, d), or (H, keys, d) for a prefix."""
-    k, v = pair
-    for t in (k, v):
-        if t.shape != shape or t.dtype != dtype:
-            raise ValueError("%s: keys and values must be %s %s, got %s %s" % (what, tuple(shape), dtype, tuple(t.shape), t.dtype))
+def _pair_source(k, v, dtype, what):
+    """(k, v) tensors (B, H, keys, d), or (H, keys, d) for a prefix -> (sid_kv_source, tensors to keep alive)."""
+    if v.shape != k.shape or k.dtype != dtype or v.dtype != dtype:
+        raise ValueError("%s: keys and values must be alike and %s, got %s %s and %s %s"
+                         % (what, dtype, tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
     k, v = _rows16(k), _rows16(v)
     ks, vs = k.stride()[:-1], v.stride()[:-1]
-    if len(shape) == 3:
+    if len(ks) == 2:
         ks, vs = (0,) + ks, (0,) + vs
-    return _lib.KVSource(k.data_ptr(), v.data_ptr(), None, None, _lib.Strides(*ks), _lib.Strides(*vs),
-                         (_lib._c.c_longlong * 2)(0, 0), _lib.KV_NONE), (k, v)
+    return _lib.kv_source(k.data_ptr(), v.data_ptr(), 0, 0, *ks, *vs, 0, 0, _lib.KV_NONE), (k, v)
 
 
 def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False, scale=None, prefix_len=None, out=None):
@@ -593,33 +609,41 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
         raise TypeError("q must be bfloat16 or float16, got %s" % q.dtype)
     B, Hq, n, d = q.shape
     _need_device(dev)
-    Hkv, P, S, src, keep = None, 0, 0, [None, None], []
-    for i, (part, what) in enumerate(((prefix, "prefix"), (own, "own part"))):
-        if part is None:
-            continue
-        if isinstance(part, QuantKV):
-            if part.B != (B if i else 1) or part.d != d:
-                raise ValueError("%s: the cache holds (B, d) = %s, the call needs %s" % (what, (part.B, part.d), (B if i else 1, d)))
-            _need_device(dev, part.k_codes)
-            heads, keys = part.H, part.S
-            src[i] = part._source()
+    P = S = 0
+    Hp = Ho = None
+    src_p = src_o = alive = None
+    if prefix is not None:
+        if isinstance(prefix, QuantKV):
+            if prefix.B != 1 or prefix.d != d:
+                raise ValueError("prefix: the cache holds (B, d) = %s, the call needs %s" % ((prefix.B, prefix.d), (1, d)))
+            _need_device(dev, prefix.k_codes)
+            Hp, P, src_p = prefix.H, prefix.S, prefix._source()
         else:
-            k, v = part
-            if k.dim() != (4 if i else 3):
-                raise ValueError("%s: keys must be %s, got %s" % (what, "(B, H, S, d)" if i else "(H, P, d)", tuple(k.shape)))
+            k, v = prefix
+            if k.dim() != 3 or k.shape[2] != d:
+                raise ValueError("prefix: keys must be (H, P, %d), got %s" % (d, tuple(k.shape)))
             _need_device(dev, k, v)
-            heads, keys = k.shape[-3], k.shape[-2]
-            src[i], alive = _pair_source(part, ((B,) if i else ()) + (heads, keys, d), q.dtype, what)
-            keep.append(alive)
-        if Hkv not in (None, heads):
-            raise ValueError("prefix and own part differ in heads: %d and %d" % (Hkv, heads))
-        Hkv = heads
-        if i:
-            S = keys
+            Hp, P = k.shape[:2]
+            src_p, alive = _pair_source(k, v, q.dtype, "prefix")
+    if own is not None:
+        if isinstance(own, QuantKV):
+            if own.B != B or own.d != d:
+                raise ValueError("own part: the cache holds (B, d) = %s, the call needs %s" % ((own.B, own.d), (B, d)))
+            _need_device(dev, own.k_codes)
+            Ho, S, src_o = own.H, own.S, own._source()
         else:
-            P = keys
+            k, v = own
+            if k.dim() != 4 or k.shape[0] != B or k.shape[3] != d:
+                raise ValueError("own part: keys must be (%d, H, S, %d), got %s" % (B, d, tuple(k.shape)))
+            _need_device(dev, k, v)
+            Ho, S = k.shape[1:3]
+            src_o, alive_o = _pair_source(k, v, q.dtype, "own part")
+            alive = (alive, alive_o)
+    Hkv = Hp if Ho is None else Ho
     if Hkv is None:
         raise ValueError("neither a prefix nor own keys")
+    if Hp not in (None, Hkv):
+        raise ValueError("prefix and own part differ in heads: %d and %d" % (Hp, Ho))
     if prefix_len is not None:
         if not 0 <= prefix_len <= P:
             raise ValueError("prefix_len %d is outside [0, %d]" % (prefix_len, P))
@@ -632,14 +656,10 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
         out = torch.empty((B, n, Hq * d), dtype=q.dtype, device=dev)
     elif out.shape != (B, n, Hq * d) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError("out must be a contiguous %s %s on %s" % ((B, n, Hq * d), q.dtype, dev))
-    nbytes = L.sid_shared_attn_workspace_bytes(B, Hq, Hkv, n, d, P, S)
-    if nbytes == 0:
-        raise _lib.SidError(-22, L.sid_last_error().decode())
-    ws = _workspace(dev, nbytes)
-    with torch.cuda.device(dev):
+    ws = _workspace(dev, _scratch_bytes("sid_shared_attn_workspace_bytes", B, Hq, Hkv, n, d, P, S))
+    with _on(dev):
         _lib.check(L.sid_shared_attn_fwd(
-            q.data_ptr(), _lib.Strides(*q.stride()[:3]), None if src[0] is None else _lib._c.addressof(src[0]),
-            None if src[1] is None else _lib._c.addressof(src[1]), None if own_len is None else own_len.data_ptr(),
+            q.data_ptr(), _lib.strides3(*q.stride()[:3]), src_p, src_o, None if own_len is None else own_len.data_ptr(),
             out.data_ptr(), B, Hq, Hkv, n, d, P, S, float(d ** -0.5 if scale is None else scale), int(causal),
             _DTYPES3[q.dtype], ws.data_ptr(), ws.numel(), _stream(dev)))
     return out
@@ -677,11 +697,8 @@ def _norm_forward(x, groups, weight, bias, eps, act):
     _need_device(dev, *[t for t in (weight, bias) if t is not None])
     y = torch.empty_like(x)
     stats = torch.empty((2, B, groups), dtype=torch.float32, device=dev)
-    nbytes = L.sid_group_norm_workspace_bytes(B, N, C, groups, _DTYPES3[x.dtype], 0)
-    if nbytes == 0:
-        raise _lib.SidError(-22, L.sid_last_error().decode())
-    ws = _workspace(dev, nbytes)
-    with torch.cuda.device(dev):
+    ws = _workspace(dev, _scratch_bytes("sid_group_norm_workspace_bytes", B, N, C, groups, _DTYPES3[x.dtype], 0))
+    with _on(dev):
         _lib.check(L.sid_group_norm_act_fwd(
             x.data_ptr(), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
             stats.data_ptr(), stats.data_ptr() + 4 * B * groups, B, N, C, groups, float(eps), _ACTS[act], _DTYPES3[x.dtype],
@@ -708,9 +725,9 @@ class _GroupNormAct(torch.autograd.Function):
         dx = torch.empty_like(x)
         dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
         db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
-        ws = _workspace(dev, L.sid_group_norm_workspace_bytes(B, N, C, G, _DTYPES3[x.dtype], 1))
+        ws = _workspace(dev, _scratch_bytes("sid_group_norm_workspace_bytes", B, N, C, G, _DTYPES3[x.dtype], 1))
         ptr = lambda t: None if t is None else t.data_ptr()
-        with torch.cuda.device(dev):
+        with _on(dev):
             _lib.check(L.sid_group_norm_act_bwd(
                 dy.data_ptr(), x.data_ptr(), ptr(weight), ptr(bias), stats.data_ptr(), stats.data_ptr() + 4 * B * G, dx.data_ptr(),
                 ptr(dw), ptr(db), B, N, C, G, _ACTS[ctx.act], _DTYPES3[x.dtype], ws.data_ptr(), ws.numel(), _stream(dev)))

@@ -1,6 +1,4 @@
 """Refusals of the 8-bit cache, shared-prefix attention and group norm: argument checks come before any GPU call."""
-import ctypes
-
 import pytest
 import torch
 
@@ -10,7 +8,7 @@ A = 1 << 20                 # an aligned address that nothing reads
 
 
 def st(*v):
-    return lib.Strides(*v)
+    return lib.strides3(*v)
 
 
 def code(rc):
@@ -49,12 +47,12 @@ def test_nothing_to_do_is_no_error():
 
 
 def source(k=A, fmt=0, stride=(640, 320, 40), scale=None):
-    return lib.KVSource(k, A, scale, scale, st(*stride), st(*stride), (ctypes.c_longlong * 2)(16, 8), fmt)
+    return lib.kv_source(k, A, scale or 0, scale or 0, *stride, *stride, 16, 8, fmt)
 
 
 def attend(q=A, B=1, Hq=4, Hkv=2, n=1, d=40, P=8, S=0, scale=1.0, dtype=1, pre=None, own=None, ws=A, ws_bytes=1 << 30, qs=(160, 40, 160), out=A):
     pre = source() if pre is None else pre
-    ref = lambda s: None if s is None or s == 0 else ctypes.addressof(s)
+    ref = lambda s: s or None
     return code(lib.load().sid_shared_attn_fwd(q, st(*qs), ref(pre), ref(own), None, out, B, Hq, Hkv, n, d, P, S, scale, 0, dtype,
                                                ws, ws_bytes, None))
 
