@@ -365,7 +365,7 @@ int sid_kv_cache_read(const void* k_codes, const void* v_codes, const float* k_s
  *   causal    not 0: query i sees its own keys j <= own_len[b] - n + i (the last query sees all of them)
  *
  * Query head h reads key/value head h / (Hq / Hkv).  One softmax over scale * q.k of the prefix and the own keys that a
- * query sees, in f32; a query that sees none gives zeros.  Keys behind own_len are never read into the result,
+ * query sees, in f32; a query that sees none gives zeros.  8-bit parts need d >= 16.  Keys behind own_len are never read into the result,
  * whatever they hold.  Products run at 16-bit operands (8-bit codes become numbers of `dtype` first), probabilities are
  * rounded to `dtype` for the second product.  A query that sees a non-finite value within 64 keys of the causal edge
  * comes out NaN in all its columns (elsewhere: in the columns of that value).
@@ -379,7 +379,8 @@ typedef struct sid_kv_source {
     int fmt;
 } sid_kv_source;
 
-size_t sid_shared_attn_workspace_bytes(int B, int Hq, int Hkv, int n, int d, int P, int S);
+/* mixed: not 0 when one of the two parts holds 16-bit numbers and the other one codes */
+size_t sid_shared_attn_workspace_bytes(int B, int Hq, int Hkv, int n, int d, int P, int S, int mixed);
 
 int sid_shared_attn_fwd(const void* q, const long long* q_stride, const sid_kv_source* prefix, const sid_kv_source* own,
                         const int* own_len, void* out, int B, int Hq, int Hkv, int n, int d, int P, int S,

@@ -59,10 +59,8 @@ __global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ 
 }
 
 struct Plan {
-    int qt, slots;
-    unsigned grid;
+    int qt, slots, groups;
     Group g[2];
-    int blocks0;
 };
 
 constexpr int kFill = 512;          // workgroups that fill the chip: two on each of 256 CUs
@@ -77,32 +75,39 @@ int splits_for(long long items, long long keys, long long fill, int least) {
     return (int)(s < 1 ? 1 : s > kMaxSlots / 2 ? kMaxSlots / 2 : s);
 }
 
-Plan make_plan(int B, int Hkv, int G, int n, int d, int P, int S) {
+// mixed: one part holds 16-bit numbers and the other one codes, so no item may walk both.
+Plan make_plan(int B, int Hkv, int G, int n, int d, int P, int S, bool mixed) {
     Plan pl{};
     const long long rows = (long long)n * G;             // of one image
+    const int unit = tile_rows(class_of(d));
     pl.qt = 1;
-    auto add = [&](int k, int tiles, int tile_rows, int splits, int per_image, int by_keys, int segs) {
-        pl.g[k] = Group{(int)((long long)Hkv * (per_image ? B : 1) * tiles * splits), tiles, splits, pl.slots, tile_rows, per_image, by_keys, segs};
+    auto add = [&](int k, int tiles, int rows_of_tile, int splits, int per_image, int by_keys, int segs) {
+        pl.g[k] = Group{(int)((long long)Hkv * (per_image ? B : 1) * tiles * splits), tiles, splits, pl.slots, rows_of_tile, per_image, by_keys, segs,
+                        Div((unsigned)tiles), Div((unsigned)splits)};
         pl.slots += splits;
+        pl.groups = k + 1;
     };
     if (rows > 64) {
         // many rows per image: each tile walks prefix and own keys
         pl.qt = two_tiles(class_of(d)) && rows > 128 ? 2 : 1;
-        const int tile = 128 * pl.qt, tiles = ceil_div(rows, tile);
+        const int tile = 4 * unit * pl.qt, tiles = ceil_div(rows, tile);
         const long long items = (long long)B * Hkv * tiles;
-        add(0, tiles, tile, splits_for(items, (long long)P + S, kFill + items / 2, 512), 1, 0, (P ? 1 : 0) | (S ? 2 : 0));
+        if (mixed && P && S) {
+            add(0, tiles, tile, splits_for(items, P, kFill + items / 2, 512), 1, 0, 1);
+            add(1, tiles, tile, splits_for(items, S, kFill + items / 2, 512), 1, 0, 2);
+        } else {
+            add(0, tiles, tile, splits_for(items, (long long)P + S, kFill + items / 2, 512), 1, 0, (P ? 1 : 0) | (S ? 2 : 0));
+        }
     } else {
         // the chip's workgroups are shared out by the keys that prefix and own parts have to walk
         const long long all = rows * B;
-        const int by_keys = all <= 32, ptile = by_keys ? 32 : 128, ptiles = ceil_div(all, ptile), otiles = ceil_div(rows, 32);
+        const int by_keys = all <= unit, ptile = by_keys ? unit : 4 * unit, ptiles = ceil_div(all, ptile), otiles = ceil_div(rows, unit);
         const long long pitems = (long long)Hkv * ptiles, oitems = (long long)B * Hkv * otiles, pwork = pitems * P, owork = oitems * S;
         int k = 0;
         if (P) add(k++, ptiles, ptile, splits_for(pitems, P, kFill * pwork / (pwork + owork) + pitems / 2, by_keys ? 128 : 256), 0, by_keys, 1);
-        if (S) add(k++, otiles, 32, splits_for(oitems, S, kFill * owork / (pwork + owork) + oitems / 2, 128), 1, 1, 2);
-        if (!k) add(0, otiles, 32, 1, 1, 1, 0);          // no keys at all: zeros
+        if (S) add(k++, otiles, unit, splits_for(oitems, S, kFill * owork / (pwork + owork) + oitems / 2, 128), 1, 1, 2);
+        if (!k) add(0, otiles, unit, 1, 1, 1, 0);        // no keys at all: zeros
     }
-    pl.blocks0 = padded(pl.g[0].items);
-    pl.grid = (unsigned)(pl.blocks0 + padded(pl.g[1].items));
     return pl;
 }
 
@@ -128,6 +133,7 @@ int check_source(const sid_kv_source* s, int keys, int d, const char* what) {
     for (long long x : st) SID_CHECK_ARG(x * es % unit == 0, "%s: rows must be %d-byte aligned", what, unit);
     for (int i = 2; i < 6; i += 3)
         SID_CHECK_ARG(st[i] >= 0 && st[i] * es < (1 << 24), "%s: distance between tokens out of range", what);
+    SID_CHECK_ARG(s->fmt == SID_KV_NONE || d >= 16, "%s: 8-bit rows need a head_dim of 16 or more", what);
     if (s->fmt != SID_KV_NONE) SID_CHECK_ARG(s->k_scale && s->v_scale, "%s: scales missing", what);
     return SID_OK;
 }
@@ -147,9 +153,9 @@ void fill_source(Source& o, const sid_kv_source* s) {
 
 using namespace sid_shared;
 
-extern "C" size_t sid_shared_attn_workspace_bytes(int B, int Hq, int Hkv, int n, int d, int P, int S) {
+extern "C" size_t sid_shared_attn_workspace_bytes(int B, int Hq, int Hkv, int n, int d, int P, int S, int mixed) {
     if (check_shape(B, Hq, Hkv, n, d, P, S)) return 0;
-    const size_t need = plan_bytes(make_plan(B, Hkv, Hq / Hkv, n, d, P, S), (long long)B * n * Hq, d);
+    const size_t need = plan_bytes(make_plan(B, Hkv, Hq / Hkv, n, d, P, S, mixed != 0), (long long)B * n * Hq, d);
     return need ? need : 256;
 }
 
@@ -165,7 +171,8 @@ extern "C" int sid_shared_attn_fwd(const void* q, const long long* q_stride, con
     if (P) if (int rc = check_source(prefix, P, d, "prefix")) return rc;
     if (S) if (int rc = check_source(own, S, d, "own part")) return rc;
 
-    const Plan pl = make_plan(B, Hkv, Hq / Hkv, n, d, P, S);
+    const bool codes[2] = {P && prefix->fmt != SID_KV_NONE, S && own->fmt != SID_KV_NONE};
+    const Plan pl = make_plan(B, Hkv, Hq / Hkv, n, d, P, S, P && S && codes[0] != codes[1]);
     const long long rows = (long long)B * n * Hq;
     const size_t need = plan_bytes(pl, rows, d);
     if (need > workspace_bytes) return sid::fail(SID_ENOMEM, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
@@ -183,10 +190,22 @@ extern "C" int sid_shared_attn_fwd(const void* q, const long long* q_stride, con
     }
     p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.n = n; p.d = d; p.P = P; p.S = S; p.causal = causal != 0;
     p.c = scale * 1.4426950408889634f;
-    p.blocks0 = pl.blocks0;
-    p.g[0] = pl.g[0]; p.g[1] = pl.g[1];
+    p.by_B = Div((unsigned)B); p.by_G = Div((unsigned)p.G); p.by_n = Div((unsigned)n);
     const hipStream_t st = (hipStream_t)stream;
-    if (int rc = dtype == SID_DTYPE_BF16 ? launch_bf16(p, pl.qt, pl.grid, st) : launch_f16(p, pl.qt, pl.grid, st)) return rc;
+    // one launch for the groups whose parts are held alike
+    for (int g = 0; g < pl.groups;) {
+        const bool c = codes[pl.g[g].segs == 2];
+        const bool both = g + 1 < pl.groups && codes[pl.g[g + 1].segs == 2] == c;
+        p.g[0] = pl.g[g];
+        p.g[1] = both ? pl.g[g + 1] : Group{};
+        p.blocks0 = padded(p.g[0].items);
+        const unsigned grid = (unsigned)(p.blocks0 + padded(p.g[1].items));
+        int rc;
+        if (dtype == SID_DTYPE_BF16) rc = c ? launch_bf16_codes(p, pl.qt, grid, st) : launch_bf16(p, pl.qt, grid, st);
+        else rc = c ? launch_f16_codes(p, pl.qt, grid, st) : launch_f16(p, pl.qt, grid, st);
+        if (rc) return rc;
+        g += both ? 2 : 1;
+    }
     if (need) {
         // quads of a row to a power of two; slots shared by up to eight threads while that leaves each one a few
         int log_q = 4, log_sg = 0;

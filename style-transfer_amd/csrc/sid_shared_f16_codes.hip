@@ -1,0 +1,6 @@
+// Instances of the shared-prefix attention kernels: half-precision queries, keys and values held in 8 bits.
+#include "sid_shared_kernel.hpp"
+
+namespace sid_shared {
+int launch_f16_codes(const Params& p, int qt, unsigned grid, hipStream_t st) { return launch_type<_Float16, true>(p, qt, grid, st); }
+}  // namespace sid_shared

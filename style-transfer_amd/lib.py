@@ -55,7 +55,7 @@ SIGNATURES = {
     "sid_masked_adain": (_i, [_vp] * 4 + [_i, _i, _vp] + [_i] * 5 + [_vp]),
     "sid_kv_cache_write": (_i, [_vp] * 10 + [_i] * 7 + [_vp]),
     "sid_kv_cache_read": (_i, [_vp] * 7 + [_i] * 7 + [_vp]),
-    "sid_shared_attn_workspace_bytes": (_sz, [_i] * 7),
+    "sid_shared_attn_workspace_bytes": (_sz, [_i] * 8),
     "sid_shared_attn_fwd": (_i, [_vp] * 6 + [_i] * 7 + [_f] + [_i] * 2 + [_vp, _sz, _vp]),
     "sid_group_norm_workspace_bytes": (_sz, [_i] * 6),
     "sid_group_norm_act_fwd": (_i, [_vp] * 6 + [_i] * 4 + [_f] + [_i] * 2 + [_vp, _sz, _vp]),

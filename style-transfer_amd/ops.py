@@ -609,6 +609,9 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
         raise TypeError("q must be bfloat16 or float16, got %s" % q.dtype)
     B, Hq, n, d = q.shape
     _need_device(dev)
+    if d == 8:                       # the kernel reads codes sixteen at a time: rows of eight become numbers first
+        prefix, own = (tuple(t[0] for t in kv_cache_read(prefix, 0, prefix.S, q.dtype)) if isinstance(prefix, QuantKV) and prefix.B == 1 else prefix,
+                       kv_cache_read(own, 0, own.S, q.dtype) if isinstance(own, QuantKV) else own)
     P = S = 0
     Hp = Ho = None
     src_p = src_o = alive = None
@@ -656,7 +659,8 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
         out = torch.empty((B, n, Hq * d), dtype=q.dtype, device=dev)
     elif out.shape != (B, n, Hq * d) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError("out must be a contiguous %s %s on %s" % ((B, n, Hq * d), q.dtype, dev))
-    ws = _workspace(dev, _scratch_bytes("sid_shared_attn_workspace_bytes", B, Hq, Hkv, n, d, P, S))
+    ws = _workspace(dev, _scratch_bytes("sid_shared_attn_workspace_bytes", B, Hq, Hkv, n, d, P, S,
+                                         int(P and S and isinstance(prefix, QuantKV) != isinstance(own, QuantKV))))
     with _on(dev):
         _lib.check(L.sid_shared_attn_fwd(
             q.data_ptr(), _lib.strides3(*q.stride()[:3]), src_p, src_o, None if own_len is None else own_len.data_ptr(),

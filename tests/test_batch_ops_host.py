@@ -63,7 +63,7 @@ def attend(q=A, B=1, Hq=4, Hkv=2, n=1, d=40, P=8, S=0, scale=1.0, dtype=1, pre=N
     (dict(q=A + 8), "16-byte"), (dict(qs=(160, 41, 160)), "16-byte"), (dict(n=0), ">= 1"), (dict(P=-1), "negative"), (dict(out=A + 2), "8-byte"),
     (dict(pre=0), "NULL"), (dict(S=8), "own part"), (dict(pre=source(k=A + 8)), "aligned"), (dict(pre=source(stride=(0, 321, 40))), "aligned"),
     (dict(pre=source(stride=(0, 320, -40))), "distance"), (dict(pre=source(stride=(0, 320, 1 << 24))), "distance"),
-    (dict(pre=source(fmt=1)), "scales"), (dict(pre=source(fmt=4)), "format"), (dict(P=1 << 30), "too many"), (dict(B=1 << 23), "too many")])
+    (dict(pre=source(fmt=1)), "scales"), (dict(d=8, pre=source(fmt=1, scale=A), qs=(32, 8, 32)), "16 or more"), (dict(pre=source(fmt=4)), "format"), (dict(P=1 << 30), "too many"), (dict(B=1 << 23), "too many")])
 def test_shared_attention_refusals(kw, text):
     rc, msg = attend(**kw)
     assert rc == -22 and text in msg, (rc, msg)
@@ -71,15 +71,17 @@ def test_shared_attention_refusals(kw, text):
 
 def test_shared_attention_workspace():
     L = lib.load()
-    need = L.sid_shared_attn_workspace_bytes(4, 8, 8, 1, 64, 8000, 100)
+    need = L.sid_shared_attn_workspace_bytes(4, 8, 8, 1, 64, 8000, 100, 0)
     assert need > 256
     src = source(stride=(0, 8000 * 64, 64))
     rc, msg = attend(B=4, Hq=8, Hkv=8, d=64, P=8000, S=100, pre=src, own=source(stride=(51200, 6400, 64)), ws_bytes=need - 1, qs=(512, 64, 512))
     assert rc == -12 and str(need) in msg
     rc, msg = attend(B=4, Hq=8, Hkv=8, d=64, P=8000, S=100, pre=src, own=source(stride=(51200, 6400, 64)), ws=A + 64, qs=(512, 64, 512))
     assert rc == -22 and "256-byte" in msg
-    assert L.sid_shared_attn_workspace_bytes(1, 8, 8, 4096, 40, 4096, 0) >= 256
-    assert L.sid_shared_attn_workspace_bytes(1, 8, 3, 1, 40, 8, 0) == 0
+    assert L.sid_shared_attn_workspace_bytes(1, 8, 8, 4096, 40, 4096, 0, 0) >= 256
+    # parts held differently are walked by items of their own, whose results are joined
+    assert L.sid_shared_attn_workspace_bytes(4, 8, 8, 4096, 40, 4096, 4096, 1) > L.sid_shared_attn_workspace_bytes(4, 8, 8, 4096, 40, 4096, 4096, 0)
+    assert L.sid_shared_attn_workspace_bytes(1, 8, 3, 1, 40, 8, 0, 0) == 0
 
 
 def norm(x=A, B=1, N=4, C=64, G=8, eps=1e-5, act=1, dtype=0, ws=A, ws_bytes=1 << 30, mean=A):

@@ -124,6 +124,13 @@ def test_cached_keys(B, Hq, Hkv, n, d, fmt):
         run(B, Hq, Hkv, n, 333, 70, d, dtype, fmt=fmt, causal=n > 1, lens=[70 - 3 * (b % 20) for b in range(B)])
 
 
+@pytest.mark.parametrize("d", [8, 16, 24, 40, 72, 136, 168, 256])
+def test_cached_keys_of_every_row_width(d):
+    """Rows of 8 (mod 16) codes, whose last sixteen overlap; a cache that ends with the last row."""
+    for n in (1, 130):
+        run(2, 2, 2, n, 45, 37, d, torch.bfloat16, fmt=("int8", "e4m3"), lens=[37, 20])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_large_logits_and_rising_keys(dtype):
     """Logits that keep growing along the keys: the softmax reference moves many times, in every tile and split."""
