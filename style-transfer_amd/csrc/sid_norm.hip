@@ -119,6 +119,23 @@ __device__ __forceinline__ void block_sum(float (&v)[K], float* sm) {
     }
 }
 
+// Sum of x over the threads of one of the workgroup's gc groups, in every thread of that group.
+constexpr int kCluster = 4;
+__device__ __forceinline__ void cluster_sum(float& x, int own, int gc, float* sm) {
+    if (gc == 1) {
+        float v[1] = {x};
+        block_sum<1>(v, sm);
+        x = v[0];
+    } else {
+        float v[kCluster];
+#pragma unroll
+        for (int k = 0; k < kCluster; ++k) v[k] = own == k ? x : 0.f;
+        block_sum<kCluster>(v, sm);
+#pragma unroll
+        for (int k = 0; k < kCluster; ++k) x = own == k ? v[k] : x;
+    }
+}
+
 // (n, mean, m2) <- (n, mean, m2) joined with (nb, meanb, m2b)
 __device__ __forceinline__ void join(float& n, float& mean, float& m2, float nb, float meanb, float m2b) {
     const float t = n + nb;
@@ -139,7 +156,10 @@ struct NormParams {
     float2* sums;                 // backward passes: [B][G] (s1, s2)
     float2* chan;                 // backward: [B][C] (dw, db) per image
     float *dw, *db;               // (C), either may be null
-    int B, N, C, G, Cg, silu, chunks, chunk_rows;
+    int B, N, C, G, Cg, silu, chunks, chunk_rows, out_rows;       // rows of a workgroup: statistics, output pass
+    int gc;                       // resident forward: groups of one workgroup
+    int fold;                     // passes: the output pass joins the chunks' group statistics itself
+    float2* gpart;                // fold: [B][chunk][G]
     float eps;
 };
 
@@ -156,15 +176,15 @@ __device__ __forceinline__ int slice_index(int items) {
 template <int DT, int VB, int NV>
 __global__ void __launch_bounds__(1024) gn_fwd_resident(NormParams p) {
     constexpr int ES = DT == SID_DTYPE_F32 ? 4 : 2, V = VB / ES;
-    __shared__ float sm[16];
-    const int item = slice_index(p.B * p.G);
-    if (item >= p.B * p.G) return;
-    const int bi = item / p.G, g = item - bi * p.G;
-    const int cv = p.Cg / V, rp = (int)blockDim.x / cv, t = threadIdx.x;
+    __shared__ float sm[16 * kCluster];
+    const int per_image = p.G / p.gc, items = p.B * per_image, item = slice_index(items);
+    if (item >= items) return;
+    const int bi = item / per_image, g0 = (item - bi * per_image) * p.gc;
+    const int cv = p.gc * p.Cg / V, rp = (int)blockDim.x / cv, t = threadIdx.x;
     const bool live = t < rp * cv;
-    const int col = t % cv, row0 = t / cv;
+    const int col = t % cv, row0 = t / cv, own = p.gc == 1 ? 0 : col * V / p.Cg;          // this thread's group of the gc
     const size_t pitch = (size_t)p.C * ES;
-    const char* src = p.x + ((size_t)bi * p.N + row0) * pitch + ((size_t)g * p.Cg + (size_t)col * V) * ES;
+    const char* src = p.x + ((size_t)bi * p.N + row0) * pitch + ((size_t)g0 * p.Cg + (size_t)col * V) * ES;
     char* dst = p.out + (src - p.x);
 
     Raw<VB> raw[NV];
@@ -181,7 +201,7 @@ __global__ void __launch_bounds__(1024) gn_fwd_resident(NormParams p) {
 #pragma unroll
             for (int e = 0; e < V; ++e) s[0] += f[e];
         }
-    block_sum<1>(s, sm);
+    cluster_sum(s[0], own, p.gc, sm);
     const float mean = s[0] * inv_n;
     s[0] = 0.f;
 #pragma unroll
@@ -192,14 +212,14 @@ __global__ void __launch_bounds__(1024) gn_fwd_resident(NormParams p) {
 #pragma unroll
             for (int e = 0; e < V; ++e) { const float d = f[e] - mean; s[0] = __builtin_fmaf(d, d, s[0]); }
         }
-    block_sum<1>(s, sm);
+    cluster_sum(s[0], own, p.gc, sm);
     const float rstd = 1.f / sqrtf(s[0] * inv_n + p.eps);
-    if (t == 0 && p.mean) { p.mean[item] = mean; p.rstd[item] = rstd; }
     if (!live) return;
+    if (row0 == 0 && col * V == own * p.Cg) { p.mean[bi * p.G + g0 + own] = mean; p.rstd[bi * p.G + g0 + own] = rstd; }
     float w[V], b[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        const int c = g * p.Cg + col * V + e;
+        const int c = g0 * p.Cg + col * V + e;
         w[e] = (p.w ? p.w[c] : 1.f) * rstd;
         b[e] = p.b ? p.b[c] : 0.f;
     }
@@ -307,7 +327,7 @@ __global__ void __launch_bounds__(1024) gn_bwd_resident(NormParams p) {
 // column t mod cv of the slab and every rp-th row of the chunk.
 struct Lane { int cv, rp, col, row, row_end; bool live; };
 template <int V>
-__device__ __forceinline__ Lane lane_of(const NormParams& p) {
+__device__ __forceinline__ Lane lane_of(const NormParams& p, int rows) {
     Lane l;
     const int cvs = p.C / V, slab0 = (int)blockIdx.z * 512;
     l.cv = min(512, cvs - slab0);
@@ -315,17 +335,25 @@ __device__ __forceinline__ Lane lane_of(const NormParams& p) {
     const int t = threadIdx.x;
     l.live = t < l.rp * l.cv;
     l.col = slab0 + t % l.cv;
-    const int r0 = (int)blockIdx.x * p.chunk_rows;
+    const int r0 = (int)blockIdx.x * rows;
     l.row = r0 + t / l.cv;
-    l.row_end = min(p.N, r0 + p.chunk_rows);
+    l.row_end = min(p.N, r0 + rows);
     return l;
+}
+
+constexpr int kFoldGroups = 512;
+// Lanes that share one group's work in a workgroup of 512: a power of two, 64 at most.
+__device__ __forceinline__ int lanes_per_group(int G) {
+    int n = 64;
+    while (n * G > 512) n >>= 1;
+    return n;
 }
 
 template <int DT, int VB>
 __global__ void __launch_bounds__(512) gn_stats(NormParams p) {
     constexpr int ES = DT == SID_DTYPE_F32 ? 4 : 2, V = VB / ES, R = 8;
     __shared__ float lm[V][512], l2[V][512], ln[512];
-    const Lane l = lane_of<V>(p);
+    const Lane l = lane_of<V>(p, p.chunk_rows);
     const size_t pitch = (size_t)p.C * ES;
     const char* src = p.x + (size_t)blockIdx.y * p.N * pitch + (size_t)l.col * VB;
     float n = 0.f, mean[V], m2[V];
@@ -400,6 +428,87 @@ __global__ void __launch_bounds__(512) gn_stats(NormParams p) {
     }
 }
 
+// Sums over the rp row threads and Cg channels of group g of what ls holds per thread and channel; in the L lanes of the group.
+template <int V>
+__device__ __forceinline__ float group_sum(const float (&ls)[V][512], const NormParams& p, const Lane& l, int g, int lane, int L) {
+    float s = 0.f;
+    if (g < p.G)
+        for (int i = lane; i < p.Cg; i += L) {
+            const int c = g * p.Cg + i;
+            const float* at = &ls[c % V][c / V];
+            for (int r = 0; r < l.rp; ++r) s += at[r * l.cv];
+        }
+    for (int off = L >> 1; off >= 1; off >>= 1) s += __shfl_xor(s, off);
+    return s;
+}
+
+// fold: (mean, centred sum) per group and chunk.  A batch of rows sits in registers: the group's mean over the workgroup,
+// then the sum of squares about it; batches join by their counts.
+template <int DT, int VB>
+__global__ void __launch_bounds__(512) gn_group_stats(NormParams p) {
+    constexpr int ES = DT == SID_DTYPE_F32 ? 4 : 2, V = VB / ES, R = 8;
+    __shared__ float ls[V][512], gm[kFoldGroups];
+    const Lane l = lane_of<V>(p, p.chunk_rows);
+    const int t = threadIdx.x, L = lanes_per_group(p.G), g = t / L, lane = t % L;
+    const size_t pitch = (size_t)p.C * ES;
+    const char* src = p.x + (size_t)blockIdx.y * p.N * pitch + (size_t)l.col * VB;
+    float n = 0.f, mean = 0.f, m2 = 0.f;
+    int of[V];                       // groups of this thread's channels
+#pragma unroll
+    for (int e = 0; e < V; ++e) of[e] = (l.col * V + e) / p.Cg;
+    for (int r0 = (int)blockIdx.x * p.chunk_rows; r0 < l.row_end; r0 += R * l.rp) {
+        const int row = r0 + t / l.cv;
+        Raw<VB> raw[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) raw[k] = load_raw<VB>(src + (size_t)min(row + k * l.rp, l.row_end - 1) * pitch);
+        float s[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+            if (l.live && row + k * l.rp < l.row_end) {
+                float f[V];
+                unpack<DT, VB>(raw[k], f);
+#pragma unroll
+                for (int e = 0; e < V; ++e) s[e] += f[e];
+            }
+#pragma unroll
+        for (int e = 0; e < V; ++e) ls[e][t] = s[e];
+        __syncthreads();
+        const float count = (float)min(l.row_end - r0, R * l.rp) * (float)p.Cg;
+        const float bm = group_sum<V>(ls, p, l, g, lane, L) / count;
+        if (g < p.G && lane == 0) gm[g] = bm;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float m = gm[of[e]];
+            float q = 0.f;
+#pragma unroll
+            for (int k = 0; k < R; ++k)
+                if (l.live && row + k * l.rp < l.row_end) {
+                    float f[V];
+                    unpack<DT, VB>(raw[k], f);
+                    const float d = f[e] - m;
+                    q = __builtin_fmaf(d, d, q);
+                }
+            ls[e][t] = q;
+        }
+        __syncthreads();
+        join(n, mean, m2, count, bm, group_sum<V>(ls, p, l, g, lane, L));
+        __syncthreads();
+    }
+    if (g < p.G && lane == 0) p.gpart[((size_t)blockIdx.y * p.chunks + blockIdx.x) * p.G + g] = make_float2(mean, m2);
+}
+
+// Joins (n, mean, m2) over the `width` lanes that share a group; the same bits in all of them.
+__device__ __forceinline__ void join_lanes(float& n, float& mean, float& m2, int width) {
+    for (int off = width >> 1; off >= 1; off >>= 1) {
+        const float nb = __shfl_xor(n, off), mb = __shfl_xor(mean, off), qb = __shfl_xor(m2, off);
+        if (threadIdx.x & off) { float a = nb, b = mb, c = qb; join(a, b, c, n, mean, m2); n = a; mean = b; m2 = c; }
+        else join(n, mean, m2, nb, mb, qb);
+    }
+}
+
 // One workgroup per (image, group): joins chunks x Cg triples into mean and rstd.
 __global__ void __launch_bounds__(256) gn_join(NormParams p) {
     __shared__ float sn[4], sm[4], s2[4];
@@ -411,13 +520,7 @@ __global__ void __launch_bounds__(256) gn_join(NormParams p) {
         const float2 v = p.part[((size_t)bi * p.chunks + ch) * p.C + (size_t)g * p.Cg + c];
         join(n, mean, m2, (float)min(p.chunk_rows, p.N - ch * p.chunk_rows), v.x, v.y);
     }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        const float nb = __shfl_xor(n, off), mb = __shfl_xor(mean, off), qb = __shfl_xor(m2, off);
-        // the same order on both sides of the exchange, so that all lanes hold the same bits
-        if (threadIdx.x & off) { float a = nb, b = mb, c = qb; join(a, b, c, n, mean, m2); n = a; mean = b; m2 = c; }
-        else join(n, mean, m2, nb, mb, qb);
-    }
+    join_lanes(n, mean, m2, 64);
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) { sn[wave] = n; sm[wave] = mean; s2[wave] = m2; }
     __syncthreads();
@@ -431,15 +534,40 @@ __global__ void __launch_bounds__(256) gn_join(NormParams p) {
 template <int DT, int VB>
 __global__ void __launch_bounds__(512) gn_apply(NormParams p) {
     constexpr int ES = DT == SID_DTYPE_F32 ? 4 : 2, V = VB / ES, R = 4;
-    const Lane l = lane_of<V>(p);
+    __shared__ float2 st[kFoldGroups];
+    const Lane l = lane_of<V>(p, p.out_rows);
+    if (p.fold) {
+        const int L = lanes_per_group(p.G), g = (int)threadIdx.x / L, lane = (int)threadIdx.x % L;
+        // the mean of the chunks' means by their rows, then the centred sums about it
+        const float2* part = p.gpart + (size_t)blockIdx.y * p.chunks * p.G + (g < p.G ? g : 0);
+        float mean = 0.f, m2 = 0.f;
+#pragma unroll 4
+        for (int ch = lane; ch < p.chunks; ch += L)
+            mean = __builtin_fmaf((float)min(p.chunk_rows, p.N - ch * p.chunk_rows), part[(size_t)ch * p.G].x, mean);
+        for (int off = L >> 1; off >= 1; off >>= 1) mean += __shfl_xor(mean, off);
+        mean /= (float)p.N;
+#pragma unroll 4
+        for (int ch = lane; ch < p.chunks; ch += L) {
+            const float2 v = part[(size_t)ch * p.G];
+            const float d = v.x - mean;
+            m2 += __builtin_fmaf((float)min(p.chunk_rows, p.N - ch * p.chunk_rows) * (float)p.Cg, d * d, v.y);
+        }
+        for (int off = L >> 1; off >= 1; off >>= 1) m2 += __shfl_xor(m2, off);
+        if (g < p.G && lane == 0) {
+            const float rstd = 1.f / sqrtf(m2 / ((float)p.N * (float)p.Cg) + p.eps);
+            st[g] = make_float2(mean, rstd);
+            if (blockIdx.x == 0) { p.mean[blockIdx.y * p.G + g] = mean; p.rstd[blockIdx.y * p.G + g] = rstd; }
+        }
+        __syncthreads();
+    }
     if (!l.live) return;
     const size_t pitch = (size_t)p.C * ES, base = (size_t)blockIdx.y * p.N * pitch + (size_t)l.col * VB;
     float mean[V], w[V], b[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int c = l.col * V + e, gi = (int)blockIdx.y * p.G + c / p.Cg;
-        mean[e] = p.mean[gi];
-        w[e] = (p.w ? p.w[c] : 1.f) * p.rstd[gi];
+        mean[e] = p.fold ? st[c / p.Cg].x : p.mean[gi];
+        w[e] = (p.w ? p.w[c] : 1.f) * (p.fold ? st[c / p.Cg].y : p.rstd[gi]);
         b[e] = p.b ? p.b[c] : 0.f;
     }
     for (int r = l.row; r < l.row_end; r += R * l.rp) {
@@ -464,7 +592,7 @@ template <int DT, int VB>
 __global__ void __launch_bounds__(512) gn_bwd_sums(NormParams p) {
     constexpr int ES = DT == SID_DTYPE_F32 ? 4 : 2, V = VB / ES, R = 4;
     __shared__ float2 ls[V][512];
-    const Lane l = lane_of<V>(p);
+    const Lane l = lane_of<V>(p, p.chunk_rows);
     const size_t pitch = (size_t)p.C * ES, base = (size_t)blockIdx.y * p.N * pitch + (size_t)l.col * VB;
     float mean[V], rstd[V], w[V], b[V], sw[V], sb[V];
 #pragma unroll
@@ -520,6 +648,20 @@ __global__ void __launch_bounds__(512) gn_bwd_sums(NormParams p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) out[e] = make_float2(sw[e], sb[e]);
     }
+    if (p.fold) {
+        const int L = lanes_per_group(p.G), g = t / L, lane = t % L;
+        float s1 = 0.f, s2 = 0.f;
+        if (g < p.G)
+            for (int c = lane; c < p.Cg; c += L) {
+                const int cc = g * p.Cg + c;
+                const float wc = p.w ? p.w[cc] : 1.f;
+                const float2 v = ls[cc % V][cc / V];
+                s1 = __builtin_fmaf(wc, v.y, s1);
+                s2 = __builtin_fmaf(wc, v.x, s2);
+            }
+        for (int off = L >> 1; off >= 1; off >>= 1) { s1 += __shfl_xor(s1, off); s2 += __shfl_xor(s2, off); }
+        if (g < p.G && lane == 0) p.gpart[((size_t)blockIdx.y * p.chunks + blockIdx.x) * p.G + g] = make_float2(s1, s2);
+    }
 }
 
 // One workgroup per (image, group): channel sums over the chunks, then the group's s1 and s2.
@@ -567,7 +709,22 @@ __global__ void __launch_bounds__(256) gn_bwd_join(NormParams p) {
 template <int DT, int VB>
 __global__ void __launch_bounds__(512) gn_bwd_apply(NormParams p) {
     constexpr int ES = DT == SID_DTYPE_F32 ? 4 : 2, V = VB / ES, R = 4;
-    const Lane l = lane_of<V>(p);
+    __shared__ float2 st[kFoldGroups];
+    const Lane l = lane_of<V>(p, p.out_rows);
+    if (p.fold) {
+        const int L = lanes_per_group(p.G), g = (int)threadIdx.x / L, lane = (int)threadIdx.x % L;
+        float a = 0.f, c = 0.f;
+        if (g < p.G)
+#pragma unroll 4
+            for (int ch = lane; ch < p.chunks; ch += L) {
+                const float2 v = p.gpart[((size_t)blockIdx.y * p.chunks + ch) * p.G + g];
+                a += v.x; c += v.y;
+            }
+        for (int off = L >> 1; off >= 1; off >>= 1) { a += __shfl_xor(a, off); c += __shfl_xor(c, off); }
+        const float inv_n = 1.f / ((float)p.N * (float)p.Cg);
+        if (g < p.G && lane == 0) st[g] = make_float2(a * inv_n, c * inv_n);
+        __syncthreads();
+    }
     if (!l.live) return;
     const size_t pitch = (size_t)p.C * ES, base = (size_t)blockIdx.y * p.N * pitch + (size_t)l.col * VB;
     float mean[V], rstd[V], w[V], b[V], s1[V], s2[V];
@@ -578,7 +735,7 @@ __global__ void __launch_bounds__(512) gn_bwd_apply(NormParams p) {
         rstd[e] = p.rstd[gi];
         w[e] = p.w ? p.w[c] : 1.f;
         b[e] = p.b ? p.b[c] : 0.f;
-        const float2 s = p.sums[gi];
+        const float2 s = p.fold ? st[c / p.Cg] : p.sums[gi];
         s1[e] = s.x; s2[e] = s.y;
     }
     for (int r = l.row; r < l.row_end; r += R * l.rp) {
@@ -606,17 +763,32 @@ __global__ void __launch_bounds__(512) gn_bwd_apply(NormParams p) {
     }
 }
 
-// dw, db: the images' channel sums in order
-__global__ void __launch_bounds__(256) gn_param_grads(const float2* chan, float* dw, float* db, int B, int C) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= C) return;
+// dw, db: `rows` rows of channel sums (images, or images x chunks), 32 channels a workgroup, every 32nd row a thread, then
+// the 32 threads of a channel in halves.
+__global__ void __launch_bounds__(1024) gn_param_grads(const float2* rows_of, float* dw, float* db, int rows, int C) {
+    __shared__ float2 ls[1024];
+    const int t = threadIdx.x, c = blockIdx.x * 32 + (t & 31), r0 = t >> 5;
     float sw = 0.f, sb = 0.f;
-    for (int b = 0; b < B; ++b) {
-        const float2 v = chan[(size_t)b * C + c];
-        sw += v.x; sb += v.y;
+    if (c < C)
+#pragma unroll 8
+        for (int r = r0; r < rows; r += 32) {
+            const float2 v = rows_of[(size_t)r * C + c];
+            sw += v.x; sb += v.y;
+        }
+    ls[t] = make_float2(sw, sb);
+    __syncthreads();
+    for (int h = 16; h >= 1; h >>= 1) {
+        if (r0 < h) {
+            const float2 o = ls[t + h * 32];
+            sw += o.x; sb += o.y;
+            ls[t] = make_float2(sw, sb);
+        }
+        __syncthreads();
     }
-    if (dw) dw[c] = sw;
-    if (db) db[c] = sb;
+    if (r0 == 0 && c < C) {
+        if (dw) dw[c] = sw;
+        if (db) db[c] = sb;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -624,7 +796,8 @@ struct Plan {
     int vb;            // bytes of one vector
     int nv;            // resident: class of vectors per thread (bytes / vb), 0 = passes
     int threads;       // resident
-    int chunks, chunk_rows;
+    int gc;            // resident forward: groups of one workgroup
+    int chunks, chunk_rows, out_rows, fold;
     size_t part_bytes, sums_bytes, chan_bytes;
 };
 
@@ -643,7 +816,11 @@ Plan make_plan(int B, int N, int C, int G, int dtype, uintptr_t addr, bool bwd) 
     const int es = dtype == SID_DTYPE_F32 ? 4 : 2, Cg = C / G;
     Plan pl{};
     const int vb = vec_bytes((long long)Cg * es, addr, es), cv = Cg * es / vb;
-    if (cv <= 1024) {
+    // Slices above 64 KB go by passes where the resident kernel's few workgroups would read them alone (forward, bf16: 64 x 64 x
+    // 320 of one image 20.5 us resident, 17.2 in passes; of four, 18.7 and 26.9) and always backward, where a thread holds two
+    // tensors (64 x 64 x 320 of sixteen images: 74 us resident, 60 in passes; of one, 36 and 24).
+    const bool large = (size_t)N * Cg * es > (64u << 10);
+    if (cv <= 1024 && !(large && (bwd || (long long)B * G <= 64))) {
         for (int threads = 256; threads <= 1024 && !pl.nv; threads *= 2) {
             if (cv > threads) continue;
             const int rows = (N + threads / cv - 1) / (threads / cv);
@@ -655,23 +832,43 @@ Plan make_plan(int B, int N, int C, int G, int dtype, uintptr_t addr, bool bwd) 
         }
     }
     pl.vb = vb;
+    pl.gc = 1;
+    if (!bwd && pl.nv) {
+        // Neighbouring groups in one workgroup while a row's piece is below a cache line, the slice still fits and there are
+        // workgroups for every CU: a piece costs an L2 request whatever its length (16 x 64 x 64 x 320, 20-byte pieces:
+        // 34.5 us with one group a workgroup, 32 with two).
+        for (int gc = 2; gc <= kCluster && G % gc == 0 && (long long)B * G / gc >= 256 && gc * cv <= 1024 && gc * Cg * es <= 128; gc *= 2) {
+            const int rows = (N + 1024 / (gc * cv) - 1) / (1024 / (gc * cv));
+            for (int i = 0; i < 3; ++i)
+                if (rows <= vectors_in(kFwdRegs[i], vb)) { pl.gc = gc; pl.threads = 1024; pl.nv = vectors_in(kFwdRegs[i], vb); break; }
+        }
+    }
     if (pl.nv) {
         pl.chan_bytes = bwd ? (size_t)B * C * sizeof(float2) : 0;
         return pl;
     }
     pl.vb = vec_bytes((long long)C * es, addr, es);
-    // chunks: about four workgroups per CU, at least 64 rows each
-    const int cvs = C * es / pl.vb, slabs = (cvs + 511) / 512;
-    long long want = 1024 / ((long long)B * slabs);
+    // Chunks: two workgroups of 512 threads for every CU, and two rows or more for every thread.  Every workgroup of the output
+    // pass joins the group statistics of its image's chunks itself, so these are 128 at most; where a row takes several
+    // workgroups, or there are more groups than threads, a launch of its own joins them.
+    const int cvs = C * es / pl.vb, slabs = (cvs + 511) / 512, rp = 512 / (cvs < 512 ? cvs : 512);
+    pl.fold = slabs == 1 && G <= kFoldGroups;
+    long long want = 512 / ((long long)B * slabs);
     if (want < 1) want = 1;
+    if (pl.fold && want > 128) want = 128;
     long long rows = (N + want - 1) / want;
-    if (rows < 64) rows = 64;
+    if (rows < 2 * rp) rows = 2 * rp;
     if (rows > N) rows = N;
     pl.chunk_rows = (int)rows;
     pl.chunks = (int)((N + rows - 1) / rows);
-    pl.part_bytes = sid::align_up((size_t)B * pl.chunks * C * sizeof(float2), 256);
-    pl.sums_bytes = bwd ? sid::align_up((size_t)B * G * sizeof(float2), 256) : 0;
-    pl.chan_bytes = bwd ? (size_t)B * C * sizeof(float2) : 0;
+    // the output pass keeps no sums: more, smaller workgroups
+    const long long out = 1024 / ((long long)B * slabs);
+    long long orows = (N + (out < 1 ? 1 : out) - 1) / (out < 1 ? 1 : out);
+    if (orows < 4 * rp) orows = 4 * rp;
+    pl.out_rows = (int)(orows > N ? N : orows);
+    pl.part_bytes = pl.fold && !bwd ? 0 : sid::align_up((size_t)B * pl.chunks * C * sizeof(float2), 256);
+    pl.sums_bytes = pl.fold ? sid::align_up((size_t)B * pl.chunks * G * sizeof(float2), 256) : bwd ? sid::align_up((size_t)B * G * sizeof(float2), 256) : 0;
+    pl.chan_bytes = bwd && !pl.fold ? (size_t)B * C * sizeof(float2) : 0;
     return pl;
 }
 
@@ -691,16 +888,21 @@ bool aligned_to_elements(uintptr_t addr, int dtype) { return addr % (dtype == SI
 template <int DT, int VB>
 int launch_fwd(const NormParams& p, const Plan& pl, hipStream_t st) {
     if (pl.nv) {
-        const dim3 grid(((p.B * p.G + kXcd - 1) / kXcd) * kXcd), block(pl.threads);
+        const int items = p.B * (p.G / p.gc);
+        const dim3 grid((items + kXcd - 1) / kXcd * kXcd), block(pl.threads);
         if (pl.nv == vectors_in(kFwdRegs[0], VB)) hipLaunchKernelGGL((gn_fwd_resident<DT, VB, vectors_in(kFwdRegs[0], VB)>), grid, block, 0, st, p);
         else if (pl.nv == vectors_in(kFwdRegs[1], VB)) hipLaunchKernelGGL((gn_fwd_resident<DT, VB, vectors_in(kFwdRegs[1], VB)>), grid, block, 0, st, p);
         else hipLaunchKernelGGL((gn_fwd_resident<DT, VB, vectors_in(kFwdRegs[2], VB)>), grid, block, 0, st, p);
     } else {
         const int cvs = p.C / (VB / (DT == SID_DTYPE_F32 ? 4 : 2));
-        const dim3 grid(pl.chunks, p.B, (cvs + 511) / 512);
-        hipLaunchKernelGGL((gn_stats<DT, VB>), grid, dim3(512), 0, st, p);
-        hipLaunchKernelGGL(gn_join, dim3(p.B * p.G), dim3(256), 0, st, p);
-        hipLaunchKernelGGL((gn_apply<DT, VB>), grid, dim3(512), 0, st, p);
+        const dim3 grid(pl.chunks, p.B, (cvs + 511) / 512), out((p.N + p.out_rows - 1) / p.out_rows, p.B, (cvs + 511) / 512);
+        if (p.fold) {
+            hipLaunchKernelGGL((gn_group_stats<DT, VB>), grid, dim3(512), 0, st, p);
+        } else {
+            hipLaunchKernelGGL((gn_stats<DT, VB>), grid, dim3(512), 0, st, p);
+            hipLaunchKernelGGL(gn_join, dim3(p.B * p.G), dim3(256), 0, st, p);
+        }
+        hipLaunchKernelGGL((gn_apply<DT, VB>), out, dim3(512), 0, st, p);
     }
     SID_CHECK_HIP(hipGetLastError());
     return SID_OK;
@@ -722,12 +924,16 @@ int launch_bwd(const NormParams& p, const Plan& pl, hipStream_t st) {
         }
     } else {
         const int cvs = p.C / (VB / (DT == SID_DTYPE_F32 ? 4 : 2));
-        const dim3 grid(pl.chunks, p.B, (cvs + 511) / 512);
+        const dim3 grid(pl.chunks, p.B, (cvs + 511) / 512), out((p.N + p.out_rows - 1) / p.out_rows, p.B, (cvs + 511) / 512);
         hipLaunchKernelGGL((gn_bwd_sums<DT, VB>), grid, dim3(512), 0, st, p);
-        hipLaunchKernelGGL(gn_bwd_join, dim3(p.B * p.G), dim3(256), 0, st, p);
-        if (p.out) hipLaunchKernelGGL((gn_bwd_apply<DT, VB>), grid, dim3(512), 0, st, p);
+        if (!p.fold) hipLaunchKernelGGL(gn_bwd_join, dim3(p.B * p.G), dim3(256), 0, st, p);
+        if (p.out) hipLaunchKernelGGL((gn_bwd_apply<DT, VB>), out, dim3(512), 0, st, p);
     }
-    if (p.chan) hipLaunchKernelGGL(gn_param_grads, dim3((p.C + 255) / 256), dim3(256), 0, st, p.chan, p.dw, p.db, p.B, p.C);
+    if (p.dw || p.db) {
+        const bool chunks = !pl.nv && p.fold;            // the chunks' sums themselves
+        hipLaunchKernelGGL(gn_param_grads, dim3((p.C + 31) / 32), dim3(1024), 0, st, chunks ? p.part : p.chan, p.dw, p.db,
+                           chunks ? p.B * p.chunks : p.B, p.C);
+    }
     SID_CHECK_HIP(hipGetLastError());
     return SID_OK;
 }
@@ -783,8 +989,10 @@ extern "C" int sid_group_norm_act_fwd(const void* x, const float* weight, const 
     SID_CHECK_ARG(plan_bytes(pl) == 0 || (workspace && (uintptr_t)workspace % 256 == 0), "workspace must be 256-byte aligned");
     NormParams p = params_of(B, N, C, G, act);
     p.x = (const char*)x; p.out = (char*)y; p.w = weight; p.b = bias; p.mean = mean; p.rstd = rstd; p.eps = eps;
-    p.chunks = pl.chunks; p.chunk_rows = pl.chunk_rows;
+    p.chunks = pl.chunks; p.chunk_rows = pl.chunk_rows; p.out_rows = pl.out_rows;
+    p.gc = pl.gc; p.fold = pl.fold;
     p.part = (float2*)workspace;
+    p.gpart = (float2*)((char*)workspace + pl.part_bytes);
     return by_dtype(p, pl, dtype, false, (hipStream_t)stream);
 }
 
@@ -802,11 +1010,12 @@ extern "C" int sid_group_norm_act_bwd(const void* dy, const void* x, const float
     NormParams p = params_of(B, N, C, G, act);
     p.x = (const char*)x; p.dy = (const char*)dy; p.out = (char*)dx; p.w = weight; p.b = bias;
     p.mean = (float*)mean; p.rstd = (float*)rstd;
-    p.chunks = pl.chunks; p.chunk_rows = pl.chunk_rows;
+    p.chunks = pl.chunks; p.chunk_rows = pl.chunk_rows; p.out_rows = pl.out_rows;
     p.dw = dweight; p.db = dbias;
     char* ws = (char*)workspace;
     p.part = (float2*)ws;
-    p.sums = (float2*)(ws + pl.part_bytes);
-    p.chan = dweight || dbias ? (float2*)(ws + pl.part_bytes + pl.sums_bytes) : nullptr;
+    p.fold = pl.fold;
+    p.sums = p.gpart = (float2*)(ws + pl.part_bytes);
+    p.chan = (dweight || dbias) && !(pl.fold && !pl.nv) ? (float2*)(ws + pl.part_bytes + pl.sums_bytes) : nullptr;
     return by_dtype(p, pl, dtype, true, (hipStream_t)stream);
 }
