@@ -10,6 +10,7 @@ them runs in libsid.so:
   mask file present, q/k injected      (:425-546)      sid_injected_attn_fwd (3 key blocks + bias)
   mask file present, nothing injected  (:556-566)      sid_plain_attn_fwd, logit scale T*scale
   no mask file, or cross-attention     (:569-579)      sid_plain_attn_fwd, T only if q or k injected
+  the same, 8-bit style keys/values (ops.QuantKV)      sid_shared_attn_fwd: one copy for the whole batch
   gen_pkl (feature extraction)         (:584-604)      torch (it must expose qk_sim / attn)
 """
 import math
@@ -137,6 +138,9 @@ class CrossAttention(nn.Module):
             side = int(math.sqrt(n))
             if side * side != n:
                 raise ValueError("token count %d is not a square grid" % n)
+            if isinstance(k_injected, ops.QuantKV):
+                raise TypeError("8-bit key/value features serve the single-style attention only; this call takes the mask-based "
+                                "path (%s exists): load the feature store without quantisation" % mask_path)
             m = self.mask_cache.signed_mask(mask_path, side, side, x.device)
             if isinstance(k_injected, ops.PackedKV):
                 # the feature store keeps the key/value pairs in the kernels' operand layout
@@ -184,6 +188,13 @@ class CrossAttention(nn.Module):
             q = torch.cat([q_injected] * b) * gamma + self._split(xq) * (1. - 0.5)     # (:376-381)
             q_layout = "bhnd"
             self.q = q
+        if use_mask:
+            logit_scale = T * self.scale                   # (:557-559)
+        else:
+            logit_scale = (T if (q_injected is not None or k_injected is not None) else 1.0) * self.scale
+        if isinstance(k_injected, ops.QuantKV):
+            self.k, self.v = k_injected, v_injected
+            return self.to_out(self._shared(q, k_injected, logit_scale, q_layout, b, compute))
         if k_injected is None:
             k, v = self.to_k(context), self.to_v(context)
             kv_layout = "bnhd"
@@ -193,10 +204,6 @@ class CrossAttention(nn.Module):
             v = torch.cat([v_injected] * b, dim=0)
             kv_layout = "bhnd"
             self.k, self.v = k, v
-        if use_mask:
-            logit_scale = T * self.scale                   # (:557-559)
-        else:
-            logit_scale = (T if (q_injected is not None or k_injected is not None) else 1.0) * self.scale
         out = self._plain(q.contiguous(), self._as(k, q), self._as(v, q), logit_scale, q_layout, kv_layout, compute)
         return self.to_out(out)
 
@@ -229,6 +236,20 @@ class CrossAttention(nn.Module):
         compute = resolve_compute(compute, n_keys, d, logit_scale)
         return ops.plain_attention(q, k, v, logit_scale, self.heads, q_layout=q_layout, kv_layout=kv_layout,
                                    compute=compute, flags=self.kernel_flags)
+
+    def _shared(self, q, kv, logit_scale, q_layout, b, compute):
+        """Single-block attention on one 8-bit copy of a style's keys and values (FeatureStore.quantize), which every image of
+        the batch reads: the reference repeats the pair b times (:577-578).  compute 'f16' / 'bf16' is the type of the queries,
+        probabilities and read-back values; 'fp32', and temperatures the shared kernel does not take, run the plain kernel on
+        the pair read back as numbers."""
+        h, d = self.heads, q.shape[-1] // (self.heads if q_layout == "bnhd" else 1)
+        compute = resolve_compute(compute, kv.S, d, logit_scale)
+        if compute == "fp32" or not logit_scale > 0:
+            k, v = (t.expand(b, -1, -1, -1).reshape(b * h, kv.S, d) for t in ops.kv_cache_read(kv, 0, kv.S, q.dtype))
+            return self._plain(q.contiguous(), k, v, logit_scale, q_layout, "bhnd", compute)
+        q16 = q.to(torch.float16 if compute == "f16" else torch.bfloat16)
+        q16 = q16.view(b, -1, h, d).transpose(1, 2) if q_layout == "bnhd" else q16.view(b, h, -1, d)
+        return ops.shared_prefix_attention(q16, kv, None, scale=logit_scale).to(q.dtype)
 
     @staticmethod
     def _as(t, like):

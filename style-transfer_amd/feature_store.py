@@ -192,6 +192,16 @@ class FeatureStore:
             cache_content_blocks(self.cnt, heads)
         return self
 
+    def quantize(self, heads=8, fmt="int8"):
+        """Convert the style list's key/value pairs of a single-style store to 8 bits (ops.QuantKV), in place:
+        `..._self_attn_k` and `..._self_attn_v` of a block then hold ONE QuantKV and the two tensors are dropped.  The
+        attention of any number of images reads the one copy (sid_shared_attn_fwd): 44 bytes a key and head at
+        head_dim 40 against 160 in float32.  fmt: "int8" or "e4m3" (ops.kv_cache)."""
+        if self.back is not None:
+            raise ValueError("8-bit key/value pairs serve the single-style attention; a two-style store is packed (pack())")
+        quantize_feature_list(self.char, heads, fmt)
+        return self
+
     def nbytes(self):
         seen, total = set(), 0
         for f in self.lists():
@@ -202,6 +212,9 @@ class FeatureStore:
                     elif hasattr(v, "image") and id(v) not in seen:
                         seen.add(id(v))
                         total += v.nbytes() + (v.partial.nbytes() if v.partial is not None else 0)
+                    elif hasattr(v, "k_codes") and id(v) not in seen:
+                        seen.add(id(v))
+                        total += v.nbytes()
         return total
 
 
@@ -216,6 +229,24 @@ def pack_feature_list(feats, heads=8, compute="f16", T=None):
             temp = T if T is not None else (entry.get("config") or {}).get("T", 1.0)
             mode = resolve_injected_compute(compute, n, d, temp, d ** -0.5)
             kv = ops.pack_kv(entry[key].contiguous(), entry[vkey].contiguous(), heads, mode)
+            entry[key] = entry[vkey] = kv
+    return feats
+
+
+def quantize_feature_list(feats, heads=8, fmt="int8"):
+    """FeatureStore.quantize for one list, in place (an already quantised or packed entry is left alone, and so is a layer
+    whose head_dim the 8-bit cache does not hold: no multiple of 8, or above 256)."""
+    from . import ops
+    for entry in feats:
+        for key in [k for k in entry if k.endswith("_self_attn_k") and torch.is_tensor(entry[k])]:
+            vkey = key[:-1] + "v"
+            k, v = entry[key], entry[vkey]
+            if k.shape[0] != heads:
+                raise ValueError("%s has %d heads, the network %d" % (key, k.shape[0], heads))
+            if k.shape[2] % 8 or k.shape[2] > 256:
+                continue
+            kv = ops.kv_cache(1, heads, k.shape[1], k.shape[2], fmt, k.device)
+            ops.kv_cache_write(kv, k[None], v[None])
             entry[key] = entry[vkey] = kv
     return feats
 

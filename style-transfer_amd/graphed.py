@@ -25,6 +25,8 @@ def _clone_slot(v):
             p = v.partial
             slot.partial = ops.ContentPartial(p.data.clone(), p.B, p.H, p.N, p.d, p.compute, p.scale, None)
         return slot
+    if isinstance(v, ops.QuantKV):
+        return ops.QuantKV(*(t.clone() for t in v.tensors()))
     if isinstance(v, dict):
         return dict(v)
     return v
@@ -37,6 +39,9 @@ def _copy_into(slot, v):
         slot.image.copy_(v.image, non_blocking=True)
         if slot.partial is not None:
             slot.partial.data.copy_(v.partial.data, non_blocking=True)
+    elif isinstance(slot, ops.QuantKV):
+        for s, t in zip(slot.tensors(), v.tensors()):
+            s.copy_(t, non_blocking=True)
 
 
 class GraphedUNet:
@@ -51,8 +56,10 @@ class GraphedUNet:
     def _signature(self, x, context, feats):
         cnt = tuple(getattr(m, "cnt_name", None) for m in self.unet.attention_modules()[:1])
         cfg = None if feats is None else (feats["config"].get("T"), feats["config"].get("gamma"))
-        # (a key is marked when its pair carries a cached content block: the evaluation then takes another entry point)
-        keys = None if feats is None else tuple(sorted(k + ("+" if getattr(v, "partial", None) is not None else "")
+        # (a key is marked when its pair carries a cached content block, or is held in 8 bits: the evaluation then takes
+        # another entry point)
+        keys = None if feats is None else tuple(sorted(k + ("+" if getattr(v, "partial", None) is not None else
+                                                            ":%d" % v.fmt if isinstance(v, ops.QuantKV) else "")
                                                        for k, v in feats.items() if k != "config"))
         return (tuple(x.shape), x.dtype, None if context is None else tuple(context.shape), cnt, cfg, keys)
 

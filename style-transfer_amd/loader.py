@@ -40,12 +40,15 @@ class FeatureLoader:
     stream."""
 
     def __init__(self, precomputed, device, heads=8, compute="f16", T=None, dtype=None, packed=True,
-                 cache_content=False, cache_bytes=96 << 30, sidecar="use", prefetch=True, staging_bytes=96 << 20):
+                 cache_content=False, cache_bytes=96 << 30, sidecar="use", prefetch=True, staging_bytes=96 << 20, quantize=None):
         if sidecar not in ("off", "use", "write"):
             raise ValueError("sidecar must be 'off', 'use' or 'write'")
         self.precomputed, self.device = precomputed, torch.device(device)
         self.heads, self.compute, self.T, self.dtype = heads, compute, T, dtype
+        if quantize not in (None, "int8", "e4m3"):
+            raise ValueError("quantize must be None, 'int8' or 'e4m3'")
         self.packed, self.cache_content = packed, cache_content
+        self.quantize = quantize                    # format of a single-style line's style list (FeatureStore.quantize)
         self.cache_bytes, self.sidecar, self.prefetch = cache_bytes, sidecar, prefetch
         self._cache = OrderedDict()                 # (role, base) -> _Loaded, least recently used first
         self._pending = {}                          # (role, base) -> Future
@@ -58,10 +61,13 @@ class FeatureLoader:
                       "routes": {"pkl": 0, "sidecar": 0}, "evicted": 0}
 
     # ---- what to load -------------------------------------------------------------------------
-    @staticmethod
-    def _keys(bases):
+    def _style_role(self, bases):
+        # a style may serve two-style lines (packed) and single-style lines (tensors, or 8 bits): two entries of the cache
+        return "sty1" if (self.packed or self.quantize) and bases[2] is None else "sty"
+
+    def _keys(self, bases):
         cnt, char, back = bases
-        keys = [("cnt", cnt), ("sty", char)]
+        keys = [("cnt", cnt), (self._style_role(bases), char)]
         if back is not None and back != char:
             keys.append(("sty", back))
         return keys
@@ -105,7 +111,7 @@ class FeatureLoader:
                     b.record_stream(cur)
         self._evict(set(got))
         cnt, char, back = bases
-        return fs.FeatureStore(got[("cnt", cnt)].feats, got[("sty", char)].feats,
+        return fs.FeatureStore(got[("cnt", cnt)].feats, got[(self._style_role(bases), char)].feats,
                                got[("sty", back)].feats if two_styles else None)
 
     def _evict(self, keep):
@@ -174,6 +180,8 @@ class FeatureLoader:
                     with ops.capture_lock, torch.cuda.stream(self._stream):
                         if want_packed and route == "pkl":
                             fs.pack_feature_list([e], self.heads, self.compute, self.T)
+                        if role == "sty1" and self.quantize:
+                            fs.quantize_feature_list([e], self.heads, self.quantize)
                         if want_packed and role == "cnt" and self.cache_content:
                             fs.cache_content_blocks([e], self.heads)
                 with ops.capture_lock:
@@ -194,7 +202,8 @@ class FeatureLoader:
         for e in feats:
             for v in e.values():
                 ts = [v] if torch.is_tensor(v) else ([v.image] + ([v.partial.data] if v.partial is not None else [])
-                                                     if isinstance(v, ops.PackedKV) else [])
+                                                     if isinstance(v, ops.PackedKV) else
+                                                     v.tensors() if isinstance(v, ops.QuantKV) else [])
                 for t in ts:
                     sp = t.untyped_storage().data_ptr()
                     if sp not in seen:

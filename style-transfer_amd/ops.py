@@ -78,6 +78,13 @@ def _workspace(device, nbytes):
     return ws
 
 
+def _call_scratch(device, nbytes):
+    """Scratch memory of this call's own, for the entry points whose launches pass partial results through it: calls of two
+    threads on one stream, and two graphs captured on one stream and replayed on different ones, never share it (a captured
+    call's lies in its graph's memory pool)."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
 def _need_cuda(*ts):
     dev = ts[0].device
     for t in ts:
@@ -495,6 +502,9 @@ class QuantKV:
         self.B, self.H, self.S, self.d = shape
         self.device, self.fmt = dev, fmt
 
+    def tensors(self):
+        return self.k_codes, self.k_scale, self.v_codes, self.v_scale
+
     def nbytes(self):
         return 2 * (self.k_codes.numel() + 4 * self.k_scale.numel())
 
@@ -659,7 +669,7 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
         out = torch.empty((B, n, Hq * d), dtype=q.dtype, device=dev)
     elif out.shape != (B, n, Hq * d) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError("out must be a contiguous %s %s on %s" % ((B, n, Hq * d), q.dtype, dev))
-    ws = _workspace(dev, _scratch_bytes("sid_shared_attn_workspace_bytes", B, Hq, Hkv, n, d, P, S,
+    ws = _call_scratch(dev, _scratch_bytes("sid_shared_attn_workspace_bytes", B, Hq, Hkv, n, d, P, S,
                                          int(P and S and isinstance(prefix, QuantKV) != isinstance(own, QuantKV))))
     with _on(dev):
         _lib.check(L.sid_shared_attn_fwd(
@@ -701,7 +711,7 @@ def _norm_forward(x, groups, weight, bias, eps, act):
     _need_device(dev, *[t for t in (weight, bias) if t is not None])
     y = torch.empty_like(x)
     stats = torch.empty((2, B, groups), dtype=torch.float32, device=dev)
-    ws = _workspace(dev, _scratch_bytes("sid_group_norm_workspace_bytes", B, N, C, groups, _DTYPES3[x.dtype], 0))
+    ws = _call_scratch(dev, _scratch_bytes("sid_group_norm_workspace_bytes", B, N, C, groups, _DTYPES3[x.dtype], 0))
     with _on(dev):
         _lib.check(L.sid_group_norm_act_fwd(
             x.data_ptr(), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
@@ -729,7 +739,7 @@ class _GroupNormAct(torch.autograd.Function):
         dx = torch.empty_like(x)
         dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
         db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
-        ws = _workspace(dev, _scratch_bytes("sid_group_norm_workspace_bytes", B, N, C, G, _DTYPES3[x.dtype], 1))
+        ws = _call_scratch(dev, _scratch_bytes("sid_group_norm_workspace_bytes", B, N, C, G, _DTYPES3[x.dtype], 1))
         ptr = lambda t: None if t is None else t.data_ptr()
         with _on(dev):
             _lib.check(L.sid_group_norm_act_bwd(

@@ -73,6 +73,11 @@ def build_parser():
                         "loaded) and reuse it, its feature list and its filtered residuals for every style pair with the "
                         "same content image: the dataset.txt lines of one content are processed next to each other, on one rank")
     p.add_argument('--unpacked_store', action='store_true', help="keep key/value features as tensors instead of the kernels' operand layout")
+    p.add_argument('--quantize_store', default='off', choices=['off', 'int8', 'e4m3'],
+                   help="single-style lines: keep the style's keys and values in 8 bits (a quarter of the float32 store), read by "
+                        "the attention as they lie there; lines with a mask keep the packed store")
+    p.add_argument('--channels_last', action='store_true',
+                   help="run the host network channels last, group norm and SiLU in one kernel (off: the stock operators)")
     p.add_argument('--lanes', type=int, default=1,
                    help="images in flight on one GPU: each lane replays its own HIP graph of the UNet evaluation on its own stream "
                         "(implies --graph_unet; lines whose content has a residual file are stylised one at a time)")
@@ -137,7 +142,8 @@ def load_unet(opt, device):
         sd = sd.get("state_dict", sd)
         pre = "model.diffusion_model."
         model.load_state_dict({k[len(pre):]: v for k, v in sd.items() if k.startswith(pre)}, strict=True)
-    return model.eval().to(device)
+    model = model.eval().to(device)
+    return model.use_channels_last() if getattr(opt, "channels_last", False) else model
 
 
 def model_heads(model):
@@ -154,6 +160,8 @@ def make_loader(opt, model, device, prefetch=None):
                          packed=packed, cache_content=packed and getattr(opt, "cache_content", False),
                          cache_bytes=int(getattr(opt, "store_cache_gb", 96.0) * (1 << 30)),
                          sidecar=getattr(opt, "sidecar", "use"),
+                         quantize=None if opt.without_attn_injection or getattr(opt, "quantize_store", "off") == "off"
+                         else opt.quantize_store,
                          prefetch=(not getattr(opt, "no_prefetch", False)) if prefetch is None else prefetch)
 
 

@@ -1,7 +1,8 @@
 """SD-v1 topology UNet that carries the injected attention: the host network around the hot path.
 
 Everything here is stock PyTorch (convolutions, GroupNorm, LayerNorm, GEGLU feed-forward) except
-the attention itself, which is `style_transfer_amd.attention.CrossAttention` (the HIP kernels).
+the attention itself, which is `style_transfer_amd.attention.CrossAttention` (the HIP kernels), and,
+after `UNetModel.use_channels_last()`, the group norms with the SiLU behind them (`ops.group_norm_act`).
 Parameter names follow the Stable Diffusion v1 checkpoint layout (`input_blocks.4.1.
 transformer_blocks.0.attn1.to_q.weight`, ...), so an SD-v1.4 state dict loads unchanged; the
 configuration is `models/ldm/stable-diffusion-v1/v1-inference.yaml:29-44` of the reference.
@@ -20,6 +21,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import ops
 from .attention import CrossAttention
 
 _ATTN_KEYS = (("q_injected", "q"), ("k_injected", "k"), ("v_injected", "v"), ("cnt_k_injected", "k_cnt"),
@@ -66,10 +68,17 @@ class GroupNorm32(nn.GroupNorm):
         return super().forward(x.float()).type(x.dtype)
 
 
+def norm_act(norm, x, act):
+    """A GroupNorm module and the activation behind it in one kernel, channels last."""
+    return ops.group_norm_act(x.contiguous(memory_format=torch.channels_last), norm.num_groups, norm.weight, norm.bias,
+                              eps=norm.eps, act=act)
+
+
 class ResBlock(nn.Module):
     """GroupNorm-SiLU-conv twice with the timestep embedding added in between.  Keeps `out_skip` and
     `out_h` of the last call: the high-frequency patch (high_frequency.py) rebuilds the block output
     from them (openaimodel.py:315-328)."""
+    fused_norm = False               # UNetModel.use_channels_last
 
     def __init__(self, channels, emb_channels, out_channels=None, dropout=0.0):
         super().__init__()
@@ -85,11 +94,12 @@ class ResBlock(nn.Module):
         return self._forward(x, emb, out_layers_injected)
 
     def _forward(self, x, emb, out_layers_injected=None):
-        h = self.in_layers(x)
+        h = self.in_layers[2](norm_act(self.in_layers[0], x, "silu")) if self.fused_norm else self.in_layers(x)
         if out_layers_injected is not None:
             h = torch.cat([out_layers_injected] * x.shape[0])
         else:
-            h = self.out_layers(h + self.emb_layers(emb).type(h.dtype)[..., None, None])
+            h = h + self.emb_layers(emb).type(h.dtype)[..., None, None]
+            h = self.out_layers[2:](norm_act(self.out_layers[0], h, "silu")) if self.fused_norm else self.out_layers(h)
         self.out_skip = self.skip_connection(x)
         self.out_h = h
         return self.out_skip + h
@@ -151,6 +161,8 @@ class BasicTransformerBlock(nn.Module):
 
 
 class SpatialTransformer(nn.Module):
+    fused_norm = False               # UNetModel.use_channels_last
+
     def __init__(self, in_channels, n_heads, d_head, depth=1, context_dim=None):
         super().__init__()
         inner = n_heads * d_head
@@ -162,7 +174,8 @@ class SpatialTransformer(nn.Module):
 
     def forward(self, x, context=None, **attn_kw):
         b, c, h, w = x.shape
-        y = self.proj_in(self.norm(x)).reshape(b, -1, h * w).transpose(1, 2)       # b (h w) c
+        y = norm_act(self.norm, x, "none") if self.fused_norm else self.norm(x)
+        y = self.proj_in(y).reshape(b, -1, h * w).transpose(1, 2)                  # b (h w) c
         for blk in self.transformer_blocks:
             y = blk(y, context=context, **attn_kw)
         y = y.transpose(1, 2).reshape(b, -1, h, w)
@@ -186,6 +199,7 @@ class Stage(nn.Sequential):
 class UNetModel(nn.Module):
     """Defaults are the SD-v1 configuration: 320 channels, multipliers (1,2,4,4), two ResBlocks per
     level, transformers at downsampling 1, 2 and 4 with 8 heads, 768-wide text context."""
+    fused_norm = False
 
     def __init__(self, in_channels=4, model_channels=320, out_channels=4, num_res_blocks=2,
                  attention_resolutions=(4, 2, 1), channel_mult=(1, 2, 4, 4), num_heads=8, context_dim=768,
@@ -226,6 +240,15 @@ class UNetModel(nn.Module):
                 self.output_blocks.append(Stage(*layers))
         self.out = nn.Sequential(GroupNorm32(32, ch), nn.SiLU(), nn.Conv2d(model_channels, out_channels, 3, padding=1))
 
+    def use_channels_last(self):
+        """Weights and activations in channels-last memory, every group norm and the SiLU behind it as one kernel
+        (ops.group_norm_act).  Parameter names and the results' meaning stay; the sums round in another order."""
+        self.to(memory_format=torch.channels_last)
+        for m in self.modules():
+            if isinstance(m, (ResBlock, SpatialTransformer, UNetModel)):
+                m.fused_norm = True
+        return self
+
     def attention_modules(self):
         return [m for m in self.modules() if isinstance(m, BasicTransformerBlock.attention_cls)]
 
@@ -244,4 +267,6 @@ class UNetModel(nn.Module):
         for i, blk in enumerate(self.output_blocks):
             kw, out_layers = route_injected(injected_features, i)
             h = blk(torch.cat([h, hs.pop()], dim=1), emb, context, out_layers_injected=out_layers, **kw)
+        if self.fused_norm:
+            return self.out[2](norm_act(self.out[0], h, "silu")).contiguous()
         return self.out(h)

@@ -1,0 +1,93 @@
+"""How the network, the feature store, the loader and the command line reach the 8-bit key/value pairs and the channels-last
+group norm: what is decided on the host, without a GPU."""
+import types
+
+import numpy as np
+import pytest
+import torch
+
+from style_transfer_amd import feature_store as fs
+from style_transfer_amd import ops
+from style_transfer_amd import run as cli
+from style_transfer_amd import unet as U
+from style_transfer_amd.attention import CrossAttention
+from style_transfer_amd.loader import FeatureLoader
+
+SMALL = dict(model_channels=32, num_heads=4, channel_mult=(1, 2), attention_resolutions=(1, 2), context_dim=16)
+
+
+def pair(heads=4, n=16, d=8):
+    return ops.kv_cache(1, heads, n, d, "int8", "cpu")
+
+
+def test_flags_are_off_by_default():
+    opt = cli.build_parser().parse_args([])
+    assert opt.quantize_store == "off" and opt.channels_last is False
+    assert cli.build_parser().parse_args(["--quantize_store", "e4m3", "--channels_last"]).quantize_store == "e4m3"
+    with pytest.raises(SystemExit):
+        cli.build_parser().parse_args(["--quantize_store", "int4"])
+
+
+@pytest.mark.parametrize("flag,off,want", [("off", False, None), ("int8", False, "int8"), ("e4m3", True, None)])
+def test_loader_is_told_the_format(flag, off, want):
+    opt = types.SimpleNamespace(precomputed="/nowhere", feature_dtype="float32", unpacked_store=False, without_attn_injection=off,
+                                compute="f16", T=1.5, quantize_store=flag)
+    loader = cli.make_loader(opt, U.UNetModel(**SMALL), "cpu", prefetch=False)
+    assert loader.quantize == want
+    loader.close()
+
+
+def test_one_style_in_both_kinds_of_lines_is_two_cache_entries():
+    loader = FeatureLoader("/nowhere", "cpu", prefetch=False, quantize="int8")
+    assert loader._keys(("c", "s", None)) == [("cnt", "c"), ("sty1", "s")]
+    assert loader._keys(("c", "s", "b")) == [("cnt", "c"), ("sty", "s"), ("sty", "b")]
+    assert loader._path(("sty1", "s")) == loader._path(("sty", "s"))
+    plain = FeatureLoader("/nowhere", "cpu", prefetch=False, packed=False)
+    assert plain._keys(("c", "s", None)) == [("cnt", "c"), ("sty", "s")]
+    with pytest.raises(ValueError, match="quantize"):
+        FeatureLoader("/nowhere", "cpu", prefetch=False, quantize="int4")
+
+
+def test_two_style_store_is_not_quantised():
+    with pytest.raises(ValueError, match="single-style"):
+        fs.FeatureStore([{}], [{}], [{}]).quantize()
+
+
+def test_head_count_is_checked():
+    feats = [{"output_block_9_self_attn_k": torch.zeros(4, 16, 8), "output_block_9_self_attn_v": torch.zeros(4, 16, 8)}]
+    with pytest.raises(ValueError, match="4 heads, the network 8"):
+        fs.quantize_feature_list(feats, heads=8)
+
+
+def test_layers_the_cache_does_not_hold_stay_tensors():
+    feats = [{"output_block_9_self_attn_k": torch.zeros(4, 16, 20), "output_block_9_self_attn_v": torch.zeros(4, 16, 20)}]
+    fs.quantize_feature_list(feats, heads=4)
+    assert torch.is_tensor(feats[0]["output_block_9_self_attn_k"])
+
+
+def test_quantised_pair_on_the_mask_path_is_refused(tmp_path):
+    np.save(str(tmp_path / "img_mask.npy"), np.ones((64, 64), np.float32))
+    attn = CrossAttention(32, heads=4, dim_head=8)
+    attn.cnt_name = str(tmp_path / "img.jpg")
+    kv = pair()
+    with pytest.raises(TypeError, match="8-bit key/value features serve the single-style attention"):
+        attn(torch.zeros(1, 16, 32), q_injected=torch.zeros(4, 16, 8), k_injected=kv, v_injected=kv)
+
+
+def test_store_counts_a_pair_once():
+    kv = pair(4, 16, 8)
+    store = fs.FeatureStore([{}], [{"output_block_9_self_attn_k": kv, "output_block_9_self_attn_v": kv}])
+    assert store.nbytes() == kv.nbytes() == 2 * 4 * 16 * (8 + 4)
+
+
+def test_channels_last_keeps_names_and_marks_every_norm():
+    model = U.UNetModel(**SMALL)
+    names = [n for n, _ in model.named_parameters()]
+    assert not any(getattr(m, "fused_norm", False) for m in model.modules())
+    assert model.use_channels_last() is model
+    assert [n for n, _ in model.named_parameters()] == names
+    marked = [m for m in model.modules() if getattr(m, "fused_norm", False)]
+    norms = [m for m in model.modules() if isinstance(m, torch.nn.GroupNorm)]
+    blocks = [m for m in marked if isinstance(m, U.ResBlock)]
+    assert len(norms) == 2 * len(blocks) + (len(marked) - len(blocks) - 1) + 1
+    assert model.input_blocks[1][0].in_layers[2].weight.is_contiguous(memory_format=torch.channels_last)
