@@ -460,15 +460,13 @@ def _need_device(dev, *ts):
 
 
 def _rows16(t):
-    """`t` (..., d) with d contiguous and every row on a 16-byte boundary: itself, or a copy."""
-    bits = t.data_ptr()
-    st = t.stride()
-    es = t.element_size()
-    for s in st[:-1]:
-        bits |= s * es
-    if st[-1] == 1 and not bits & 15:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    """`t` (..., d) with d contiguous and every row on a 16-byte boundary (itself, or a copy), its address, its strides."""
+    st, ptr = t.stride(), t.data_ptr()
+    steps = st[0] | st[1] | st[-2]                       # of three or four dimensions
+    if st[-1] != 1 or (ptr | steps * t.element_size()) & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        return t, t.data_ptr(), t.stride()
+    return t, ptr, st
 
 
 @functools.lru_cache(maxsize=4096)
@@ -557,9 +555,10 @@ def kv_cache_write(cache, k, v, start=0, length=None):
         length = _positions(length, B, dev)
         _need_device(dev, length)
     _need_device(dev, k, v, start)
-    k, v = _rows16(k), _rows16(v)
+    k, kp, ks = _rows16(k)
+    v, vp, vs = _rows16(v)
     with _on(dev):
-        _lib.check(L.sid_kv_cache_write(k.data_ptr(), v.data_ptr(), _lib.strides3(*k.stride()[:3]), _lib.strides3(*v.stride()[:3]),
+        _lib.check(L.sid_kv_cache_write(kp, vp, _lib.strides3(*ks[:3]), _lib.strides3(*vs[:3]),
                                         cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scale.data_ptr(),
                                         cache.v_scale.data_ptr(), start.data_ptr(), None if length is None else length.data_ptr(),
                                         B, H, n, cache.S, d, _DTYPES3[k.dtype], cache.fmt, _stream(dev)))
@@ -593,11 +592,11 @@ def _pair_source(k, v, dtype, what):
     if v.shape != k.shape or k.dtype != dtype or v.dtype != dtype:
         raise ValueError("%s: keys and values must be alike and %s, got %s %s and %s %s"
                          % (what, dtype, tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
-    k, v = _rows16(k), _rows16(v)
-    ks, vs = k.stride()[:-1], v.stride()[:-1]
-    if len(ks) == 2:
-        ks, vs = (0,) + ks, (0,) + vs
-    return _lib.kv_source(k.data_ptr(), v.data_ptr(), 0, 0, *ks, *vs, 0, 0, _lib.KV_NONE), (k, v)
+    k, kp, ks = _rows16(k)
+    v, vp, vs = _rows16(v)
+    if len(ks) == 3:
+        return _lib.kv_source(kp, vp, 0, 0, 0, ks[0], ks[1], 0, vs[0], vs[1], 0, 0, _lib.KV_NONE), (k, v)
+    return _lib.kv_source(kp, vp, 0, 0, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], 0, 0, _lib.KV_NONE), (k, v)
 
 
 def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False, scale=None, prefix_len=None, out=None):
@@ -664,7 +663,7 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
     if own_len is not None:
         own_len = _positions(own_len, B, dev)
         _need_device(dev, own_len)
-    q = _rows16(q)
+    q, qp, qs = _rows16(q)
     if out is None:
         out = torch.empty((B, n, Hq * d), dtype=q.dtype, device=dev)
     elif out.shape != (B, n, Hq * d) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
@@ -673,7 +672,7 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
                                          int(P and S and isinstance(prefix, QuantKV) != isinstance(own, QuantKV))))
     with _on(dev):
         _lib.check(L.sid_shared_attn_fwd(
-            q.data_ptr(), _lib.strides3(*q.stride()[:3]), src_p, src_o, None if own_len is None else own_len.data_ptr(),
+            qp, _lib.strides3(qs[0], qs[1], qs[2]), src_p, src_o, None if own_len is None else own_len.data_ptr(),
             out.data_ptr(), B, Hq, Hkv, n, d, P, S, float(d ** -0.5 if scale is None else scale), int(causal),
             _DTYPES3[q.dtype], ws.data_ptr(), ws.numel(), _stream(dev)))
     return out
@@ -699,31 +698,47 @@ def _norm_shape(x, groups):
     raise ValueError("x must be (B, C, H, W) in channels-last memory or (B, N, C), got %s" % (tuple(x.shape),))
 
 
-def _norm_forward(x, groups, weight, bias, eps, act):
+def _norm_forward(x, groups, weight, bias, eps, act, keep):
+    """-> y and, for a backward pass (`keep`), the float32 mean and rstd (2, B, groups)."""
     L = _lib.load()
     dev = x.device
     B, N, C = _norm_shape(x, groups)
-    if x.dtype not in _DTYPES3:
+    dt = _DTYPES3.get(x.dtype)
+    if dt is None:
         raise TypeError("x must be float32, bfloat16 or float16, got %s" % x.dtype)
-    for t in (weight, bias):
-        if t is not None and (t.shape != (C,) or t.dtype != torch.float32 or not t.is_contiguous()):
-            raise ValueError("weight and bias must be contiguous float32 (C,) = (%d,)" % C)
-    _need_device(dev, *[t for t in (weight, bias) if t is not None])
+    wp = bp = None
+    if weight is not None:
+        _norm_param(dev, weight, C)
+        wp = weight.data_ptr()
+    if bias is not None:
+        _norm_param(dev, bias, C)
+        bp = bias.data_ptr()
+    _need_device(dev)
     y = torch.empty_like(x)
-    stats = torch.empty((2, B, groups), dtype=torch.float32, device=dev)
-    ws = _call_scratch(dev, _scratch_bytes("sid_group_norm_workspace_bytes", B, N, C, groups, _DTYPES3[x.dtype], 0))
+    need = _scratch_bytes("sid_group_norm_workspace_bytes", B, N, C, groups, dt, 0)
+    half = 4 * B * groups
+    if keep:
+        ws, stats = _call_scratch(dev, need), torch.empty((2, B, groups), dtype=torch.float32, device=dev)
+        sp = stats.data_ptr()
+    else:                                    # one allocation for both: the scratch memory first, it wants the alignment
+        ws, stats = _call_scratch(dev, (need + 3) // 4 * 4 + 2 * half), None
+        sp = ws.data_ptr() + (need + 3) // 4 * 4
     with _on(dev):
-        _lib.check(L.sid_group_norm_act_fwd(
-            x.data_ptr(), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
-            stats.data_ptr(), stats.data_ptr() + 4 * B * groups, B, N, C, groups, float(eps), _ACTS[act], _DTYPES3[x.dtype],
-            ws.data_ptr(), ws.numel(), _stream(dev)))
+        _lib.check(L.sid_group_norm_act_fwd(x.data_ptr(), wp, bp, y.data_ptr(), sp, sp + half, B, N, C, groups, float(eps),
+                                            _ACTS[act], dt, ws.data_ptr(), need, _stream(dev)))
     return y, stats
+
+
+def _norm_param(dev, t, C):
+    if t.shape != (C,) or t.dtype != torch.float32 or not t.is_contiguous():
+        raise ValueError("weight and bias must be contiguous float32 (C,) = (%d,)" % C)
+    _need_device(dev, t)
 
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        y, stats = _norm_forward(x, groups, weight, bias, eps, act)
+        y, stats = _norm_forward(x, groups, weight, bias, eps, act, True)
         ctx.save_for_backward(x, weight, bias, stats)
         ctx.groups, ctx.act = groups, act
         return y
@@ -760,6 +775,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="silu"):
         weight = weight.float()
     if bias is not None and bias.dtype != torch.float32:
         bias = bias.float()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
+                                    or bias is not None and bias.requires_grad):
         return _GroupNormAct.apply(x, weight, bias, groups, eps, act)
-    return _norm_forward(x, groups, weight, bias, eps, act)[0]
+    return _norm_forward(x, groups, weight, bias, eps, act, False)[0]

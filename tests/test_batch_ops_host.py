@@ -152,8 +152,9 @@ def test_python_layer_refuses_wrong_shapes_and_types():
 
 def test_rows_are_copied_only_between_16_byte_boundaries():
     t = torch.zeros(2, 3, 4, 48, dtype=torch.bfloat16)
-    assert ops._rows16(t) is t
+    assert ops._rows16(t) [1:] == (t.data_ptr(), t.stride()) and ops._rows16(t)[0] is t
     view = t.transpose(1, 2)
-    assert ops._rows16(view) is view
+    assert ops._rows16(view)[0] is view
     odd = torch.zeros(2, 3, 4, 49, dtype=torch.bfloat16)[..., 1:]
-    assert ops._rows16(odd) is not odd and ops._rows16(odd).is_contiguous()
+    got, ptr, strides = ops._rows16(odd)
+    assert got is not odd and got.is_contiguous() and ptr == got.data_ptr() and strides == got.stride()
