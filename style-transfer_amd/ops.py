@@ -699,7 +699,8 @@ def _norm_shape(x, groups):
 
 
 def _norm_forward(x, groups, weight, bias, eps, act, keep):
-    """-> y and, for a backward pass (`keep`), the float32 mean and rstd (2, B, groups)."""
+    """-> y and, for a backward pass (`keep`), a tensor that holds the float32 mean and rstd (2, B, groups) from a byte
+    offset on, that offset and the sizes of the call."""
     L = _lib.load()
     dev = x.device
     B, N, C = _norm_shape(x, groups)
@@ -716,17 +717,17 @@ def _norm_forward(x, groups, weight, bias, eps, act, keep):
     _need_device(dev)
     y = torch.empty_like(x)
     need = _scratch_bytes("sid_group_norm_workspace_bytes", B, N, C, groups, dt, 0)
-    half = 4 * B * groups
-    if keep:
-        ws, stats = _call_scratch(dev, need), torch.empty((2, B, groups), dtype=torch.float32, device=dev)
-        sp = stats.data_ptr()
+    half, at = 4 * B * groups, (need + 3) // 4 * 4
+    if keep and need > 65536:                # what the backward pass keeps alive is the statistics alone
+        ws, stats, at = _call_scratch(dev, need), _call_scratch(dev, 2 * half), 0
     else:                                    # one allocation for both: the scratch memory first, it wants the alignment
-        ws, stats = _call_scratch(dev, (need + 3) // 4 * 4 + 2 * half), None
-        sp = ws.data_ptr() + (need + 3) // 4 * 4
+        ws = stats = _call_scratch(dev, at + 2 * half)
+    sp = stats.data_ptr() + at
+    act = _ACTS[act]
     with _on(dev):
-        _lib.check(L.sid_group_norm_act_fwd(x.data_ptr(), wp, bp, y.data_ptr(), sp, sp + half, B, N, C, groups, float(eps),
-                                            _ACTS[act], dt, ws.data_ptr(), need, _stream(dev)))
-    return y, stats
+        _lib.check(L.sid_group_norm_act_fwd(x.data_ptr(), wp, bp, y.data_ptr(), sp, sp + half, B, N, C, groups, eps, act, dt,
+                                            ws.data_ptr(), need, _stream(dev)))
+    return y, stats, (at, B, N, C, groups, act, dt)
 
 
 def _norm_param(dev, t, C):
@@ -735,32 +736,44 @@ def _norm_param(dev, t, C):
     _need_device(dev, t)
 
 
+def _norm_backward(ctx, dy):
+    """Runs on autograd's own thread, which wakes up for it on a core that may be slow: nothing is decided here that the
+    forward pass knew."""
+    x, weight, bias, stats = ctx.saved_tensors
+    at, B, N, C, G, act, dt = ctx.call
+    dev = x.device
+    if dy.dtype != x.dtype or dy.stride() != x.stride():
+        dy = dy.to(x.dtype).contiguous(memory_format=torch.channels_last if x.dim() == 4 else torch.contiguous_format)
+    _, need_w, need_b = ctx.needs_input_grad[:3]
+    dx = torch.empty_like(x)
+    dw = torch.empty_like(weight) if need_w else None
+    db = torch.empty_like(bias) if need_b else None
+    need = _scratch_bytes("sid_group_norm_workspace_bytes", B, N, C, G, dt, 1)
+    ws = _call_scratch(dev, need)
+    sp = stats.data_ptr() + at
+    with _on(dev):
+        _lib.check(_lib.load().sid_group_norm_act_bwd(
+            dy.data_ptr(), x.data_ptr(), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
+            sp, sp + 4 * B * G, dx.data_ptr(), dw.data_ptr() if need_w else None, db.data_ptr() if need_b else None,
+            B, N, C, G, act, dt, ws.data_ptr(), need, _stream(dev)))
+    return dx, dw, db, None, None, None
+
+
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        y, stats = _norm_forward(x, groups, weight, bias, eps, act, True)
+        y, stats, ctx.call = _norm_forward(x, groups, weight, bias, eps, act, True)
         ctx.save_for_backward(x, weight, bias, stats)
-        ctx.groups, ctx.act = groups, act
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        L = _lib.load()
-        dev, G = x.device, ctx.groups
-        B, N, C = _norm_shape(x, G)
-        dy = dy.to(x.dtype).contiguous(memory_format=torch.channels_last if x.dim() == 4 else torch.contiguous_format)
-        dx = torch.empty_like(x)
-        dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
-        db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
-        ws = _call_scratch(dev, _scratch_bytes("sid_group_norm_workspace_bytes", B, N, C, G, _DTYPES3[x.dtype], 1))
-        ptr = lambda t: None if t is None else t.data_ptr()
-        with _on(dev):
-            _lib.check(L.sid_group_norm_act_bwd(
-                dy.data_ptr(), x.data_ptr(), ptr(weight), ptr(bias), stats.data_ptr(), stats.data_ptr() + 4 * B * G, dx.data_ptr(),
-                ptr(dw), ptr(db), B, N, C, G, _ACTS[ctx.act], _DTYPES3[x.dtype], ws.data_ptr(), ws.numel(), _stream(dev)))
-        return dx, dw, db, None, None, None
+        if torch.is_grad_enabled():          # create_graph: the result refuses a second derivative
+            return _norm_backward_once(ctx, dy)
+        return _norm_backward(ctx, dy)
+
+
+_norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward)
 
 
 def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="silu"):
@@ -771,6 +784,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="silu"):
     weight and bias and all arithmetic are float32; y has x's dtype and memory order.  Needs at least one value."""
     if act not in _ACTS:
         raise ValueError("act must be 'silu' or 'none', got %r" % (act,))
+    eps = float(eps)
     if weight is not None and weight.dtype != torch.float32:
         weight = weight.float()
     if bias is not None and bias.dtype != torch.float32:

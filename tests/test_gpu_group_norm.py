@@ -207,3 +207,29 @@ def test_another_stream_while_the_first_is_busy():
                 outs.append(o.group_norm_act(x, 2, w, b))
     torch.cuda.synchronize()
     assert all(torch.equal(t, want) for t in outs)
+
+
+def test_second_derivative_is_refused():
+    """create_graph gives the gradients; differentiating them again is an error, not a silent zero."""
+    x = torch.randn(2, 6, 8, device="cuda:0", requires_grad=True)
+    w = torch.randn(8, device="cuda:0", requires_grad=True)
+    y = ops().group_norm_act(x, 2, w)
+    want = torch.autograd.grad(y, (x, w), torch.ones_like(y), retain_graph=True)
+    got = torch.autograd.grad(y, (x, w), torch.ones_like(y), create_graph=True)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError):
+        got[0].square().sum().backward()
+
+
+def test_gradient_in_another_order_or_type():
+    """An incoming gradient that is expanded, strided or of another type gives what its contiguous copy gives."""
+    torch.manual_seed(9)
+    x = torch.randn(2, 6, 5, 8, device="cuda:0").permute(0, 3, 1, 2).requires_grad_()
+    y = ops().group_norm_act(x, 4)
+    g = torch.randn(2, 8, 6, 5, device="cuda:0")
+    want = torch.autograd.grad(y, x, g.contiguous(memory_format=torch.channels_last), retain_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(y, x, g, retain_graph=True)[0], want)
+    one = torch.ones((), device="cuda:0").expand(2, 8, 6, 5)
+    want = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(y, x, one, retain_graph=True)[0], want)

@@ -11,6 +11,7 @@ done
 wait
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o exp/diag.so $OBJ/sid_common.cpp.o exp/d_sid_attn.o exp/d_sid_attn_bf16.o exp/d_sid_attn_x3.o exp/d_sid_attn_f16.o exp/d_sid_attn_wide.o \
   $OBJ/sid_attn_small.hip.o $OBJ/sid_mask.hip.o $OBJ/sid_hf.hip.o $OBJ/sid_adain.hip.o $OBJ/sid_kv.hip.o $OBJ/sid_norm.hip.o \
-  $OBJ/sid_shared.hip.o $OBJ/sid_shared_bf16.hip.o $OBJ/sid_shared_f16.hip.o
+  $OBJ/sid_shared.hip.o $OBJ/sid_shared_bf16.hip.o $OBJ/sid_shared_f16.hip.o \
+  $OBJ/sid_shared_bf16_codes.hip.o $OBJ/sid_shared_f16_codes.hip.o
 rm exp/d_*.o
 echo exp/diag.so
