@@ -89,14 +89,19 @@ Plan make_plan(int B, int Hkv, int G, int n, int d, int P, int S, bool mixed) {
     };
     if (rows > 64) {
         // many rows per image: each tile walks prefix and own keys
-        pl.qt = two_tiles(class_of(d)) && rows > 128 ? 2 : 1;
+        auto items_of = [&](int qt) { return (long long)B * Hkv * ceil_div(rows, 4 * unit * qt); };
+        auto splits_of = [&](long long items, long long keys) { return splits_for(items, keys, kFill + items / 2, 512); };
+        // 64 rows a wave read every fragment of the keys once for two tiles (d = 40, 4 x 4096 queries: 246 us, 274 with 32), as
+        // long as the chip is full all the same (8 x 256 queries on 512 keys, 128 workgroups: 15 us, 10.5 with 32)
+        const long long twos = items_of(2);
+        pl.qt = two_tiles(class_of(d)) && twos * splits_of(twos, (long long)P + S) >= kFill ? 2 : 1;
         const int tile = 4 * unit * pl.qt, tiles = ceil_div(rows, tile);
-        const long long items = (long long)B * Hkv * tiles;
+        const long long items = items_of(pl.qt);
         if (mixed && P && S) {
-            add(0, tiles, tile, splits_for(items, P, kFill + items / 2, 512), 1, 0, 1);
-            add(1, tiles, tile, splits_for(items, S, kFill + items / 2, 512), 1, 0, 2);
+            add(0, tiles, tile, splits_of(items, P), 1, 0, 1);
+            add(1, tiles, tile, splits_of(items, S), 1, 0, 2);
         } else {
-            add(0, tiles, tile, splits_for(items, (long long)P + S, kFill + items / 2, 512), 1, 0, (P ? 1 : 0) | (S ? 2 : 0));
+            add(0, tiles, tile, splits_of(items, (long long)P + S), 1, 0, (P ? 1 : 0) | (S ? 2 : 0));
         }
     } else {
         // the chip's workgroups are shared out by the keys that prefix and own parts have to walk

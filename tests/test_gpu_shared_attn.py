@@ -269,3 +269,14 @@ def test_streams_do_not_share_scratch():
                 outs.append(o.shared_prefix_attention(q, pre))
     torch.cuda.synchronize()
     assert all(torch.equal(t, want) for t in outs)
+
+
+@pytest.mark.parametrize("fmt", [("none", "none"), ("int8", "int8"), ("none", "e4m3")])
+@pytest.mark.parametrize("d", [24, 40, 56, 64])
+def test_many_rows_on_a_full_chip(d, fmt):
+    """Enough rows for 512 workgroups of 256: a wave keeps two tiles of queries.  Row tails, grouped heads, ragged lengths, the
+    causal order, and the keys of a prefix split in two."""
+    dtype = TYPES[d // 8 % 2]
+    run(32, 16, 16, 150, 77, 40, d, dtype, fmt=fmt, causal=True, lens=[(7 * b) % 43 - 1 for b in range(32)])
+    run(64, 16, 8, 70, 65, 0, d, dtype, fmt=fmt)
+    run(16, 16, 16, 131, 1100, 0, d, dtype, fmt=fmt)
