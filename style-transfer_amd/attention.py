@@ -243,6 +243,8 @@ class CrossAttention(nn.Module):
         probabilities and read-back values; 'fp32', and temperatures the shared kernel does not take, run the plain kernel on
         the pair read back as numbers."""
         h, d = self.heads, q.shape[-1] // (self.heads if q_layout == "bnhd" else 1)
+        if (kv.B, kv.H) != (1, h):
+            raise ValueError("the 8-bit pair holds (B, heads) = %s, the layer needs %s" % ((kv.B, kv.H), (1, h)))
         compute = resolve_compute(compute, kv.S, d, logit_scale)
         if compute == "fp32" or not logit_scale > 0:
             k, v = (t.expand(b, -1, -1, -1).reshape(b * h, kv.S, d) for t in ops.kv_cache_read(kv, 0, kv.S, q.dtype))

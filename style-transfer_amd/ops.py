@@ -609,7 +609,7 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
         own_len: int32 (B,) tensor on the device, how many of its own keys each sequence has (clamped to [0, S]).
         causal: query i of a sequence sees its own keys j <= own_len - n + i.
     Hq must be a multiple of Hkv (query head h reads key/value head h // (Hq // Hkv)).  scale: d ** -0.5 if None.
-    -> (B, n, Hq*d) of q's dtype.  A query that sees no key gives zeros."""
+    -> (B, n, Hq*d) of q's dtype.  A query that sees no key gives zeros.  Forward only, like the attention calls above."""
     L = _lib.load()
     dev = q.device
     if q.dim() != 4:

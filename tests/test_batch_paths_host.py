@@ -91,3 +91,11 @@ def test_channels_last_keeps_names_and_marks_every_norm():
     blocks = [m for m in marked if isinstance(m, U.ResBlock)]
     assert len(norms) == 2 * len(blocks) + (len(marked) - len(blocks) - 1) + 1
     assert model.input_blocks[1][0].in_layers[2].weight.is_contiguous(memory_format=torch.channels_last)
+
+
+def test_pair_of_other_heads_is_refused():
+    attn = CrossAttention(64, heads=8, dim_head=8)
+    attn.cnt_name = "/nowhere/img.jpg"
+    kv = pair(heads=4)
+    with pytest.raises(ValueError, match="the layer needs"):
+        attn(torch.zeros(1, 16, 64), k_injected=kv, v_injected=kv)

@@ -130,6 +130,32 @@ def test_channels_last_network_equals_the_stock_one():
     assert rel_err(out[1].cpu().numpy(), out[0].cpu().numpy()) < 1e-3
 
 
+def test_high_frequency_patch_channels_last():
+    """The patched decoder blocks add HF(h_cnt) to what a channels-last block leaves, as to what the stock one leaves."""
+    from style_transfer_amd.high_frequency import patch_decoder_resblocks_h_and_cnt_hf, unpatch_decoder_resblocks
+    from style_transfer_amd.sampler import capture_residuals, last_resblocks
+    x = torch.from_numpy(synth.normal(8400, (1, 4, 16, 16))).to(DEV)
+    ctx = torch.from_numpy(synth.normal(8500, (1, 77, 768), sigma=0.5)).to(DEV)
+    t = torch.tensor([481], device=DEV)
+    out, bare = [], None
+    for cl in (False, True):
+        model = build(cl)
+        for a in model.attention_modules():
+            a.compute = "fp32"
+        with torch.no_grad():
+            bare = model(x, t, ctx)
+            residuals = {481: capture_residuals(model)}
+            patch_decoder_resblocks_h_and_cnt_hf(model, {481}, residuals, ratio=0.3)
+            for _, m in last_resblocks(model):
+                m.ri_timestep = 481
+            try:
+                out.append(model(x, t, ctx))
+            finally:
+                unpatch_decoder_resblocks(model)
+    assert rel_err(out[1].cpu().numpy(), out[0].cpu().numpy()) < 1e-3
+    assert rel_err(out[1].cpu().numpy(), bare.cpu().numpy()) > 1e-2          # the patch does something
+
+
 def test_resblock_gradients_channels_last():
     """Forward and every gradient of a ResBlock against 64 bits; the convolutions sum up to 9 * 96 products in float32:
     sqrt(864) * 2^-24 relative a layer, far below 1e-4."""
