@@ -28,9 +28,9 @@
 // exactly; their scale multiplies the f32 logits, because a rounding of the keys would shift a logit by 2^-9 of the sum of
 // |q k|, twice the error of everything else at |logit| = 5), value codes times their scale, rounded once.
 //
-// Measured: 4 images of 4096 queries, 8 heads of 40, 4096 + 4096 keys 221 us, 670 TFLOP/s (bound by the exponentials and
+// Measured: 4 images of 4096 queries, 8 heads of 40, 4096 + 4096 keys 231 us, 743 TFLOP/s (bound by the exponentials and
 // conversions beside the products); one token of 32 sequences, 32 / 8 heads of 128, 32768 + 1024 keys 50 us + 6 us to join,
-// 4.2 TB/s (bound by memory); five tokens of 16 sequences on int8 codes, 16 / 4 heads of 128, 8191 + 333 keys 28 us + 5 us,
+// 4.2 TB/s (bound by memory); five tokens of 16 sequences on int8 codes, 16 / 4 heads of 128, 8191 + 333 keys 27 us + 5 us,
 // one token of 4 sequences on 1023 + 128 keys 8.8 us (both bound by one workgroup's chain of loads, products and join).
 #pragma once
 #include "sid_common.h"
@@ -349,6 +349,10 @@ struct Rows32 {
             }
             __builtin_amdgcn_sched_barrier(kVector);
         }
+        // Two waves share a SIMD and left alone run in step, both at the products, then both at the softmax.  The one that has its
+        // logits goes first until half of its second product is issued; the other one's products then fill the matrix unit
+        // beside its exponentials (d = 40, 4 x 4096 queries on 8192 keys: 251 -> 231 us; with 32 rows a wave it gains nothing).
+        if (QT == 2) __builtin_amdgcn_s_setprio(1);
         // V^T fragments: lane 16 a + x of a half reads row x / 4, columns 4 (x % 4) .. of a block of 4 keys and 16 columns
         const int x = lane & 15;
         const T* vb = vl + (4 * hi + (x >> 2)) * D::VSTR + ((lane >> 4) & 1) * 16 + (x & 3) * 4;
@@ -425,6 +429,7 @@ struct Rows32 {
         }
 #pragma unroll
         for (int w = 0; w < 2 * NS; ++w) {
+            if (QT == 2 && w == NS) __builtin_amdgcn_s_setprio(0);
             if (w + 1 < 2 * NS) read_v(w + 1);
             __builtin_amdgcn_sched_barrier(kVector);
 #pragma unroll
@@ -580,7 +585,7 @@ __device__ __forceinline__ void store4(char* p, float a, float b, float c, float
     *(T4*)p = v;
 }
 
-struct Item { int h, b, row_begin, row_end, L, TP, v0, v1, slot; };
+struct Item { int h, b, row_begin, row_end, L, TP, v0, v1, slot, per_image; };
 
 // Key range of the item in tiles of KT keys: first the prefix's, then the own ones.
 __device__ __forceinline__ bool find_item(const Params& p, Item& it, bool& keys_way) {
@@ -591,6 +596,7 @@ __device__ __forceinline__ bool find_item(const Params& p, Item& it, bool& keys_
     int w = (i % kXcd) * share + i / kXcd;
     if (w >= g.items || i / kXcd >= share) return false;
     keys_way = g.keys_way;
+    it.per_image = g.per_image;
     int q = g.by_tiles(w);
     const int tile = w - q * g.tiles;
     w = q;
@@ -657,6 +663,10 @@ __device__ __forceinline__ void rows_way(const Params& p, const Item& it, char* 
     if (S::kAhead && t < t1) st.load(p, s, t * 64, tid);
     R.init(p, it.h, wave_row, it.row_end, lane, it.L);                            // while the first tile is on its way
     clear_pads<T, KS, ONES>(p, kl, vl, tid & 127, tid >> 7);
+    // With 32 rows a wave the same by workgroup: of the two on a CU (i and i + 256) the later goes first (d = 128: 586 -> 574 us;
+    // five tokens of 16 sequences on codes 33.0 -> 32.1).  Not where 16-bit keys stream past the rows of all images (one token
+    // of 32 sequences 44.3 -> 45.5), nor above d = 128, where it changes nothing.
+    if (QT == 1 && !D::kWide && (CODES || it.per_image) && (blockIdx.x >> 8 & 1)) __builtin_amdgcn_s_setprio(1);
     int buf = 0;
     for (;;) {
         const int seen = seg ? least : p.P;              // tiles that end before it need no mask
