@@ -28,8 +28,8 @@
 // exactly; their scale multiplies the f32 logits, because a rounding of the keys would shift a logit by 2^-9 of the sum of
 // |q k|, twice the error of everything else at |logit| = 5), value codes times their scale, rounded once.
 //
-// Measured: 4 images of 4096 queries, 8 heads of 40, 4096 + 4096 keys 231 us, 743 TFLOP/s (bound by the exponentials and
-// conversions beside the products); one token of 32 sequences, 32 / 8 heads of 128, 32768 + 1024 keys 50 us + 6 us to join,
+// Measured: 4 images of 4096 queries, 8 heads of 40, 4096 + 4096 keys 224 us, 765 TFLOP/s (bound by the exponentials and
+// conversions beside the products; d = 128 550 us, 1000 TFLOP/s); one token of 32 sequences, 32 / 8 heads of 128, 32768 + 1024 keys 50 us + 6 us to join,
 // 4.2 TB/s (bound by memory); five tokens of 16 sequences on int8 codes, 16 / 4 heads of 128, 8191 + 333 keys 27 us + 5 us,
 // one token of 4 sequences on 1023 + 128 keys 8.8 us (both bound by one workgroup's chain of loads, products and join).
 #pragma once
