@@ -18,7 +18,7 @@
 // so a large mean costs no digits.  No atomics: sums have one order, results repeat bit for bit.
 // Measured (bf16): forward 8 x 64 x 64 x 960 resident 32 us, 3.9 TB/s; 16 x 64 x 64 x 320 32 us, 2.6 TB/s (40-byte row
 // pieces); 8 x 8 x 1280 f32 4.2 us.  Backward 8 x 64 x 64 x 960 by passes 84 us: sums 31 us at 4.1 TB/s, output 41 us at
-// 4.7 TB/s, gradients of w and b 4 us; 2 x 16 x 16 x 640 resident 7.6 us + 2.8 us.
+// 4.7 TB/s, gradients of w and b 4 us; 2 x 16 x 16 x 640 resident 7.6 us + 2.8 us (one image: no second launch).
 #include "sid_common.h"
 
 #include <cstdint>
@@ -157,7 +157,7 @@ struct NormParams {
     float *mean, *rstd;           // (B, G): written by the forward, read by the backward
     float2* part;                 // passes: [B][chunk][C]; resident backward: [B][C]
     float2* sums;                 // backward passes: [B][G] (s1, s2)
-    float2* chan;                 // backward: [B][C] (dw, db) per image
+    float2* chan;                 // backward: [B][C] (dw, db) per image; null: one image, whose sums are the gradients
     float *dw, *db;               // (C), either may be null
     int B, N, C, G, Cg, silu, chunks, chunk_rows, out_rows;       // rows of a workgroup: statistics, output pass
     int gc;                       // resident forward: groups of one workgroup
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(1024) gn_bwd_resident(NormParams p) {
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < V; ++e) { s[0] = __builtin_fmaf(w[e], sb[e], s[0]); s[1] = __builtin_fmaf(w[e], sw[e], s[1]); }
-    if (p.chan)
+    if (p.dw || p.db)
 #pragma unroll
         for (int e = 0; e < V; ++e) lds2[e * blockDim.x + t] = make_float2(sw[e], sb[e]);
     block_sum<2>(s, sm);                            // its barriers also order the channel sums above
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(1024) gn_bwd_resident(NormParams p) {
                 }
                 store_raw<VB>(p.out + at + (size_t)k * rp * pitch, pack<DT, VB>(f));
             }
-    if (!p.chan) return;
+    if (!p.dw && !p.db) return;
     // channel sums over the rp row threads, halving: thread t keeps the sums of rows t/cv, t/cv + h, ...
     for (int n = rp; n > 1;) {
         const int h = (n + 1) / 2;
@@ -322,7 +322,16 @@ __global__ void __launch_bounds__(1024) gn_bwd_resident(NormParams p) {
     }
     if (t < cv)
 #pragma unroll
-        for (int e = 0; e < V; ++e) p.chan[(size_t)bi * p.C + g * p.Cg + t * V + e] = lds2[e * blockDim.x + t];
+        for (int e = 0; e < V; ++e) {
+            const float2 a = lds2[e * blockDim.x + t];
+            const int c = g * p.Cg + t * V + e;
+            if (p.chan) {
+                p.chan[(size_t)bi * p.C + c] = a;
+            } else {
+                if (p.dw) p.dw[c] = a.x;
+                if (p.db) p.db[c] = a.y;
+            }
+        }
 }
 
 // ------------------------------------------------------------------------------------------------ passes
@@ -847,7 +856,9 @@ Plan make_plan(int B, int N, int C, int G, int dtype, uintptr_t addr, bool bwd) 
         }
     }
     if (pl.nv) {
-        pl.chan_bytes = bwd ? (size_t)B * C * sizeof(float2) : 0;
+        // one image's sums are the gradients: a launch less (16 x 16 x 640 forward and backward 12.9 -> 11.6 us).  Walking two
+        // images in one workgroup to the same end costs more than the launch (13.1 -> 14.3 us; 2 x 32 x 32 x 320 18 -> 28 us).
+        pl.chan_bytes = bwd && B > 1 ? (size_t)B * C * sizeof(float2) : 0;
         return pl;
     }
     pl.vb = vec_bytes((long long)C * es, addr, es);
@@ -915,7 +926,7 @@ template <int DT, int VB>
 int launch_bwd(const NormParams& p, const Plan& pl, hipStream_t st) {
     if (pl.nv) {
         const dim3 grid(((p.B * p.G + kXcd - 1) / kXcd) * kXcd), block(pl.threads);
-        const size_t lds = p.chan ? (size_t)pl.threads * (VB / (DT == SID_DTYPE_F32 ? 4 : 2)) * sizeof(float2) : 0;
+        const size_t lds = p.dw || p.db ? (size_t)pl.threads * (VB / (DT == SID_DTYPE_F32 ? 4 : 2)) * sizeof(float2) : 0;
         if (pl.nv == vectors_in(kBwdRegs[0], VB)) {
             int rc = sid::allow_dynamic_lds<gn_bwd_resident<DT, VB, vectors_in(kBwdRegs[0], VB)>>(65536);
             if (rc) return rc;
@@ -932,7 +943,7 @@ int launch_bwd(const NormParams& p, const Plan& pl, hipStream_t st) {
         if (!p.fold) hipLaunchKernelGGL(gn_bwd_join, dim3(p.B * p.G), dim3(256), 0, st, p);
         if (p.out) hipLaunchKernelGGL((gn_bwd_apply<DT, VB>), out, dim3(512), 0, st, p);
     }
-    if (p.dw || p.db) {
+    if ((p.dw || p.db) && !(pl.nv && p.B == 1)) {
         const bool chunks = !pl.nv && p.fold;            // the chunks' sums themselves
         hipLaunchKernelGGL(gn_param_grads, dim3((p.C + 31) / 32), dim3(1024), 0, st, chunks ? p.part : p.chan, p.dw, p.db,
                            chunks ? p.B * p.chunks : p.B, p.C);
@@ -1019,6 +1030,6 @@ extern "C" int sid_group_norm_act_bwd(const void* dy, const void* x, const float
     p.part = (float2*)ws;
     p.fold = pl.fold;
     p.sums = p.gpart = (float2*)(ws + pl.part_bytes);
-    p.chan = (dweight || dbias) && !(pl.fold && !pl.nv) ? (float2*)(ws + pl.part_bytes + pl.sums_bytes) : nullptr;
+    p.chan = pl.chan_bytes && (dweight || dbias) ? (float2*)(ws + pl.part_bytes + pl.sums_bytes) : nullptr;
     return by_dtype(p, pl, dtype, true, (hipStream_t)stream);
 }

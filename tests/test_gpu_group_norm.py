@@ -233,3 +233,16 @@ def test_gradient_in_another_order_or_type():
     one = torch.ones((), device="cuda:0").expand(2, 8, 6, 5)
     want = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)[0]
     assert torch.equal(torch.autograd.grad(y, x, one, retain_graph=True)[0], want)
+
+
+@pytest.mark.parametrize("B,H,W,C,G", [(1, 8, 8, 64, 4), (2, 8, 8, 64, 4), (1, 100, 90, 96, 1), (2, 70, 64, 320, 8)])
+def test_only_some_gradients(B, H, W, C, G):
+    """Weight's, bias's or the input's gradient alone is what it is among all three (one image and several, in registers and by
+    passes)."""
+    x, w, b, dy = make(B, H, W, C, torch.float32, 5)
+    every = [t.clone(memory_format=torch.preserve_format).requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(ops().group_norm_act(every[0], G, *every[1:]), every, dy)
+    for i in range(3):
+        some = [t.detach().requires_grad_(k == i) for k, t in enumerate(every)]
+        got = torch.autograd.grad(ops().group_norm_act(some[0], G, *some[1:]), some[i], dy)[0]
+        assert torch.equal(got, want[i])
