@@ -379,7 +379,7 @@ typedef struct sid_kv_source {
     int fmt;
 } sid_kv_source;
 
-/* mixed: not 0 when one of the two parts holds 16-bit numbers and the other one codes */
+/* mixed: not 0 when the two parts are held in different formats */
 size_t sid_shared_attn_workspace_bytes(int B, int Hq, int Hkv, int n, int d, int P, int S, int mixed);
 
 int sid_shared_attn_fwd(const void* q, const long long* q_stride, const sid_kv_source* prefix, const sid_kv_source* own,

@@ -75,7 +75,7 @@ int splits_for(long long items, long long keys, long long fill, int least) {
     return (int)(s < 1 ? 1 : s > kMaxSlots / 2 ? kMaxSlots / 2 : s);
 }
 
-// mixed: one part holds 16-bit numbers and the other one codes, so no item may walk both.
+// mixed: the parts are held in different formats, so no item may walk both.
 Plan make_plan(int B, int Hkv, int G, int n, int d, int P, int S, bool mixed) {
     Plan pl{};
     const long long rows = (long long)n * G;             // of one image
@@ -150,7 +150,6 @@ void fill_source(Source& o, const sid_kv_source* s) {
     o.kb = s->k_stride[0] * es; o.kh = s->k_stride[1] * es; o.kn = (int)(s->k_stride[2] * es);
     o.vb = s->v_stride[0] * es; o.vh = s->v_stride[1] * es; o.vn = (int)(s->v_stride[2] * es);
     o.sb = s->scale_stride[0]; o.sh = s->scale_stride[1];
-    o.fmt = s->fmt;
 }
 
 }  // namespace
@@ -176,8 +175,8 @@ extern "C" int sid_shared_attn_fwd(const void* q, const long long* q_stride, con
     if (P) if (int rc = check_source(prefix, P, d, "prefix")) return rc;
     if (S) if (int rc = check_source(own, S, d, "own part")) return rc;
 
-    const bool codes[2] = {P && prefix->fmt != SID_KV_NONE, S && own->fmt != SID_KV_NONE};
-    const Plan pl = make_plan(B, Hkv, Hq / Hkv, n, d, P, S, P && S && codes[0] != codes[1]);
+    const int fmt[2] = {P ? prefix->fmt : SID_KV_NONE, S ? own->fmt : SID_KV_NONE};
+    const Plan pl = make_plan(B, Hkv, Hq / Hkv, n, d, P, S, P && S && fmt[0] != fmt[1]);
     const long long rows = (long long)B * n * Hq;
     const size_t need = plan_bytes(pl, rows, d);
     if (need > workspace_bytes) return sid::fail(SID_ENOMEM, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
@@ -199,15 +198,15 @@ extern "C" int sid_shared_attn_fwd(const void* q, const long long* q_stride, con
     const hipStream_t st = (hipStream_t)stream;
     // one launch for the groups whose parts are held alike
     for (int g = 0; g < pl.groups;) {
-        const bool c = codes[pl.g[g].segs == 2];
-        const bool both = g + 1 < pl.groups && codes[pl.g[g + 1].segs == 2] == c;
+        const int f = fmt[pl.g[g].segs == 2];
+        const bool both = g + 1 < pl.groups && fmt[pl.g[g + 1].segs == 2] == f;
         p.g[0] = pl.g[g];
         p.g[1] = both ? pl.g[g + 1] : Group{};
         p.blocks0 = padded(p.g[0].items);
         const unsigned grid = (unsigned)(p.blocks0 + padded(p.g[1].items));
         int rc;
-        if (dtype == SID_DTYPE_BF16) rc = c ? launch_bf16_codes(p, pl.qt, grid, st) : launch_bf16(p, pl.qt, grid, st);
-        else rc = c ? launch_f16_codes(p, pl.qt, grid, st) : launch_f16(p, pl.qt, grid, st);
+        if (dtype == SID_DTYPE_BF16) rc = f != SID_KV_NONE ? launch_bf16_codes(p, f, pl.qt, grid, st) : launch_bf16(p, pl.qt, grid, st);
+        else rc = f != SID_KV_NONE ? launch_f16_codes(p, f, pl.qt, grid, st) : launch_f16(p, pl.qt, grid, st);
         if (rc) return rc;
         g += both ? 2 : 1;
     }

@@ -59,7 +59,6 @@ struct Source {                      // keys and values of the prefix, or of the
     long long kb, kh, vb, vh;        // bytes from image to image, head to head
     long long sb, sh;                // the same for the scales, in floats
     int kn, vn;                      // bytes from key to key
-    int fmt;                         // SID_KV_NONE: the call's 16-bit type
 };
 
 struct Div {                         // division by a host constant: n / d for 0 <= n < 2^31
@@ -145,7 +144,7 @@ template <int KS> struct Dims {
 struct Stream {
     const char *k, *v;
     const float *ks, *vs;
-    int kn, vn, fmt, end;            // keys from `end` on are not there
+    int kn, vn, end;                 // keys from `end` on are not there
 
     __device__ __forceinline__ Stream(const Params& p, int seg, int b, int h, int keys) {
         const Source& s = p.src[seg];
@@ -154,7 +153,7 @@ struct Stream {
         v = s.v + bi * s.vb + h * s.vh;
         ks = s.ks + bi * s.sb + h * s.sh;
         vs = s.vs + bi * s.sb + h * s.sh;
-        kn = s.kn; vn = s.vn; fmt = s.fmt; end = keys;
+        kn = s.kn; vn = s.vn; end = keys;
     }
 };
 
@@ -163,9 +162,10 @@ struct Stream {
 // one): a write to a register that an earlier load may still fill waits for that load, and so for the whole latency, and
 // where two paths meet the compiler copies what one of them loaded, which waits as well.  store_v()
 // clears what was not there; the logits of such keys are masked.
-template <typename T, int KS, int NT, int KT, bool CODES>
+template <typename T, int KS, int NT, int KT, int FMT>
 struct Stager {
     using D = Dims<KS>;
+    static constexpr bool CODES = FMT != SID_KV_NONE;
     // 16 bytes of every RPP-th row.  Codes: a lane takes 16 of them (half as many lanes a row, half as many loads), the last
     // one of a row those that end it, so rows of 8 (mod 16) codes overlap there and nothing is read behind a row.
     static constexpr int LANES = CODES ? D::LPR / 2 : D::LPR, RPP = NT / LANES, NJ = KT / RPP, NC = CODES ? NJ : 1;
@@ -201,10 +201,13 @@ struct Stager {
     }
 
     // eight codes as numbers of type T, times `scale`
-    static __device__ __forceinline__ u32x4 numbers(uint32_t w0, uint32_t w1, int fmt, float scale) {
+    static __device__ __forceinline__ u32x4 numbers(uint32_t w0, uint32_t w1, float scale) {
         float f[8];
+        // the words as they are from here on: seen through, the compiler would hold every byte in a register of its own from
+        // the load on (389 registers)
+        asm("" : "+v"(w0), "+v"(w1));
         const uint32_t w[2] = {w0, w1};
-        if (fmt == SID_KV_INT8) {
+        if constexpr (FMT == SID_KV_INT8) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(w[e / 4] >> (8 * (e & 3)));
         } else {
@@ -220,15 +223,15 @@ struct Stager {
         return __builtin_bit_cast(u32x4, o);
     }
 
-    __device__ __forceinline__ void store_k(const Params& p, int fmt, T* kl, float* scale, int t) {
+    __device__ __forceinline__ void store_k(const Params& p, T* kl, float* scale, int t) {
         const int row = t / LANES, col = col_of(p, t);
         if (!CODES && t % LANES * 8 >= p.d) return;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             T* to = kl + (row + j * RPP) * D::KSTR + col;
             if (CODES) {
-                *(u32x4*)to = numbers(k[j].x, k[j].y, fmt, 1.f);
-                *(u32x4*)(to + 8) = numbers(k[j].z, k[j].w, fmt, 1.f);
+                *(u32x4*)to = numbers(k[j].x, k[j].y, 1.f);
+                *(u32x4*)(to + 8) = numbers(k[j].z, k[j].w, 1.f);
                 if (t % LANES == 0) scale[row + j * RPP] = ks[j % NC] * p.c;
             } else {
                 *(u32x4*)to = k[j];
@@ -238,21 +241,28 @@ struct Stager {
 
     // `edge`: keys that some rows of the tile do not see are in it.  Their probability is zero, but zero times an
     // infinity or a NaN is not: such values become zeros and the key is flagged (rows that do see it turn NaN).
-    __device__ __forceinline__ void store_v(const Params& p, int fmt, T* vl, bool edge, int* bad, int t) {
+    __device__ __forceinline__ void store_v(const Params& p, T* vl, bool edge, int* bad, int t) {
         const int row = t / LANES, col = col_of(p, t);
         if (!CODES && t % LANES * 8 >= p.d) return;
-        // All but a part's last tiles need neither test of put_v (heads of 160: 468 -> 431 us).  Codes keep one path: two for
-        // them cost more than 256 registers.
-        if (!CODES && !edge && left >= KT) {
+        // all but a part's last tiles need neither test of put_v (heads of 160: 468 -> 431 us)
+        if (!edge && left >= KT) {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) *(u32x4*)(vl + (row + j * RPP) * D::VSTR + col) = v[j];
+            for (int j = 0; j < NJ; ++j) {
+                T* to = vl + (row + j * RPP) * D::VSTR + col;
+                if (CODES) {
+                    *(u32x4*)to = numbers(v[j].x, v[j].y, vs[j % NC]);
+                    *(u32x4*)(to + 8) = numbers(v[j].z, v[j].w, vs[j % NC]);
+                } else {
+                    *(u32x4*)to = v[j];
+                }
+            }
             return;
         }
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             if (CODES) {
-                put_v(vl, row + j * RPP, col, numbers(v[j].x, v[j].y, fmt, vs[j % NC]), edge, bad);
-                put_v(vl, row + j * RPP, col + 8, numbers(v[j].z, v[j].w, fmt, vs[j % NC]), edge, bad);
+                put_v(vl, row + j * RPP, col, numbers(v[j].x, v[j].y, vs[j % NC]), edge, bad);
+                put_v(vl, row + j * RPP, col + 8, numbers(v[j].z, v[j].w, vs[j % NC]), edge, bad);
             } else {
                 put_v(vl, row + j * RPP, col, v[j], edge, bad);
             }
@@ -651,10 +661,11 @@ __device__ __forceinline__ int item_query(const Params& p, const Item& it) {
     return tok - p.by_n(tok) * p.n;
 }
 
-template <typename T, int KS, int QT, bool ONES, bool CODES>
+template <typename T, int KS, int QT, bool ONES, int FMT>
 __device__ __forceinline__ void rows_way(const Params& p, const Item& it, char* lds) {
+    constexpr bool CODES = FMT != SID_KV_NONE;
     using D = Dims<KS>;
-    using S = Stager<T, KS, 256, 64, CODES>;
+    using S = Stager<T, KS, 256, 64, FMT>;
     T* kl = (T*)lds;
     T* vl = kl + D::KELEMS;
     float* scales = (float*)(lds + D::kRowData);
@@ -685,9 +696,9 @@ __device__ __forceinline__ void rows_way(const Params& p, const Item& it, char* 
                 __syncthreads();
             }
             if (!S::kAhead) st.load_k(p, s, key0, tid);
-            st.store_k(p, s.fmt, kl + buf * D::KSTR, scales + buf, tid);
+            st.store_k(p, kl + buf * D::KSTR, scales + buf, tid);
             if (!S::kAhead) st.load_v(p, s, key0, tid);
-            st.store_v(p, s.fmt, vl + buf * D::VSTR, edge, flags + buf, tid);
+            st.store_v(p, vl + buf * D::VSTR, edge, flags + buf, tid);
             __syncthreads();                             // also: every wave is done with the other buffer
             if (S::kAhead && t + 1 < t1) st.load(p, s, key0 + 64, tid);
 #pragma unroll
@@ -730,10 +741,11 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
-template <typename T, int KS, bool ONES, bool CODES>
+template <typename T, int KS, bool ONES, int FMT>
 __device__ __forceinline__ void keys_way(const Params& p, const Item& it, char* lds) {
+    constexpr bool CODES = FMT != SID_KV_NONE;
     using D = Dims<KS>;
-    using S = Stager<T, KS, 64, 32, CODES>;
+    using S = Stager<T, KS, 64, 32, FMT>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), buf = wave * 32;
     T *k = (T*)lds + buf * D::KSTR, *v = (T*)lds + D::KELEMS + buf * D::VSTR;             // this wave's own rows
     float* scales = (float*)(lds + D::kRowData) + buf;
@@ -757,9 +769,9 @@ __device__ __forceinline__ void keys_way(const Params& p, const Item& it, char* 
             wave_sync();
         }
         if (!S::kAhead) st.load_k(p, s, key0, lane);
-        st.store_k(p, s.fmt, k, scales, lane);
+        st.store_k(p, k, scales, lane);
         if (!S::kAhead) st.load_v(p, s, key0, lane);
-        st.store_v(p, s.fmt, v, edge, flags, lane);
+        st.store_v(p, v, edge, flags, lane);
         wave_sync();
         if (S::kAhead && t + 4 < t1) st.load(p, s, key0 + 128, lane);
         R.template tile<1, CODES>(p, k, v, scales, seg, key0, masked, edge, flags, lane);
@@ -805,21 +817,21 @@ __device__ __forceinline__ void keys_way(const Params& p, const Item& it, char* 
 }
 
 // QT > 1: items share rows only (many rows per image); QT == 1: either way, by the item's group.
-template <typename T, int KS, int QT, bool ONES, bool CODES>
+template <typename T, int KS, int QT, bool ONES, int FMT>
 __global__ void __launch_bounds__(256, KS <= 8 ? 2 : 1) shared_kernel(Params p) {
     extern __shared__ __align__(16) char lds[];
     Item it;
     bool by_keys;
     if (!find_item(p, it, by_keys)) return;
-    if (QT == 1 && by_keys) keys_way<T, KS, ONES, CODES>(p, it, lds);
-    else rows_way<T, KS, QT, ONES, CODES>(p, it, lds);
+    if (QT == 1 && by_keys) keys_way<T, KS, ONES, FMT>(p, it, lds);
+    else rows_way<T, KS, QT, ONES, FMT>(p, it, lds);
 }
 
-template <typename T, int KS, int QT, bool ONES, bool CODES>
+template <typename T, int KS, int QT, bool ONES, int FMT>
 int launch(const Params& p, unsigned grid, hipStream_t st) {
     using D = Dims<KS>;
-    if (int rc = sid::allow_dynamic_lds<shared_kernel<T, KS, QT, ONES, CODES>>(D::kLds)) return rc;
-    hipLaunchKernelGGL((shared_kernel<T, KS, QT, ONES, CODES>), dim3(grid), dim3(256), D::kLds, st, p);
+    if (int rc = sid::allow_dynamic_lds<shared_kernel<T, KS, QT, ONES, FMT>>(D::kLds)) return rc;
+    hipLaunchKernelGGL((shared_kernel<T, KS, QT, ONES, FMT>), dim3(grid), dim3(256), D::kLds, st, p);
     SID_CHECK_HIP(hipGetLastError());
     return SID_OK;
 }
@@ -833,25 +845,25 @@ inline int class_of(int d) {
 constexpr bool two_tiles(int ks) { return ks <= 4; }      // 64 rows per wave fit in the registers
 constexpr int tile_rows(int ks) { return ks <= 8 ? 32 : 16; }
 
-template <typename T, bool CODES>
+template <typename T, int FMT>
 int launch_type(const Params& p, int qt, unsigned grid, hipStream_t st) {
     const bool ones = p.d < 32 * ((class_of(p.d) + 1) / 2);
     switch (class_of(p.d)) {
-        case 3: return qt == 2 ? launch<T, 3, 2, true, CODES>(p, grid, st) : launch<T, 3, 1, true, CODES>(p, grid, st);
+        case 3: return qt == 2 ? launch<T, 3, 2, true, FMT>(p, grid, st) : launch<T, 3, 1, true, FMT>(p, grid, st);
         case 4:
-            if (ones) return qt == 2 ? launch<T, 4, 2, true, CODES>(p, grid, st) : launch<T, 4, 1, true, CODES>(p, grid, st);
-            return qt == 2 ? launch<T, 4, 2, false, CODES>(p, grid, st) : launch<T, 4, 1, false, CODES>(p, grid, st);
-        case 5: return launch<T, 5, 1, true, CODES>(p, grid, st);
-        case 8: return ones ? launch<T, 8, 1, true, CODES>(p, grid, st) : launch<T, 8, 1, false, CODES>(p, grid, st);
-        case 10: return launch<T, 10, 1, false, CODES>(p, grid, st);
-        default: return launch<T, 16, 1, false, CODES>(p, grid, st);
+            if (ones) return qt == 2 ? launch<T, 4, 2, true, FMT>(p, grid, st) : launch<T, 4, 1, true, FMT>(p, grid, st);
+            return qt == 2 ? launch<T, 4, 2, false, FMT>(p, grid, st) : launch<T, 4, 1, false, FMT>(p, grid, st);
+        case 5: return launch<T, 5, 1, true, FMT>(p, grid, st);
+        case 8: return ones ? launch<T, 8, 1, true, FMT>(p, grid, st) : launch<T, 8, 1, false, FMT>(p, grid, st);
+        case 10: return launch<T, 10, 1, false, FMT>(p, grid, st);
+        default: return launch<T, 16, 1, false, FMT>(p, grid, st);
     }
 }
 
 // One unit each: bf16 and f16, parts of 16-bit numbers and parts of codes.
 int launch_bf16(const Params& p, int qt, unsigned grid, hipStream_t st);
 int launch_f16(const Params& p, int qt, unsigned grid, hipStream_t st);
-int launch_bf16_codes(const Params& p, int qt, unsigned grid, hipStream_t st);
-int launch_f16_codes(const Params& p, int qt, unsigned grid, hipStream_t st);
+int launch_bf16_codes(const Params& p, int fmt, int qt, unsigned grid, hipStream_t st);
+int launch_f16_codes(const Params& p, int fmt, int qt, unsigned grid, hipStream_t st);
 
 }  // namespace sid_shared

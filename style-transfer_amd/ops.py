@@ -624,12 +624,13 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
     P = S = 0
     Hp = Ho = None
     src_p = src_o = alive = None
+    fmt_p = fmt_o = _lib.KV_NONE
     if prefix is not None:
         if isinstance(prefix, QuantKV):
             if prefix.B != 1 or prefix.d != d:
                 raise ValueError("prefix: the cache holds (B, d) = %s, the call needs %s" % ((prefix.B, prefix.d), (1, d)))
             _need_device(dev, prefix.k_codes)
-            Hp, P, src_p = prefix.H, prefix.S, prefix._source()
+            Hp, P, src_p, fmt_p = prefix.H, prefix.S, prefix._source(), prefix.fmt
         else:
             k, v = prefix
             if k.dim() != 3 or k.shape[2] != d:
@@ -642,7 +643,7 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
             if own.B != B or own.d != d:
                 raise ValueError("own part: the cache holds (B, d) = %s, the call needs %s" % ((own.B, own.d), (B, d)))
             _need_device(dev, own.k_codes)
-            Ho, S, src_o = own.H, own.S, own._source()
+            Ho, S, src_o, fmt_o = own.H, own.S, own._source(), own.fmt
         else:
             k, v = own
             if k.dim() != 4 or k.shape[0] != B or k.shape[3] != d:
@@ -669,7 +670,7 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
     elif out.shape != (B, n, Hq * d) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError("out must be a contiguous %s %s on %s" % ((B, n, Hq * d), q.dtype, dev))
     ws = _call_scratch(dev, _scratch_bytes("sid_shared_attn_workspace_bytes", B, Hq, Hkv, n, d, P, S,
-                                         int(P and S and isinstance(prefix, QuantKV) != isinstance(own, QuantKV))))
+                                         int(P and S and fmt_p != fmt_o)))
     with _on(dev):
         _lib.check(L.sid_shared_attn_fwd(
             qp, _lib.strides3(qs[0], qs[1], qs[2]), src_p, src_o, None if own_len is None else own_len.data_ptr(),
