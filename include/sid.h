@@ -356,7 +356,7 @@ int sid_kv_cache_read(const void* k_codes, const void* v_codes, const float* k_s
 /*
  * Attention of a batch that shares a prefix of keys and values.
  * The reference's single-style path repeats the injected keys and values for every image of a batch
- * (ldm/modules/attention.py:389-401, torch.cat([k_injected] * b)); here the prefix exists once.
+ * (the no-mask branch, ldm/modules/attention.py:569-579); here the prefix exists once.
  *
  *   q         (B, Hq, n, d)        out  (B, n, Hq*d) contiguous      bf16 or f16
  *   prefix    P keys and values (Hkv, P, d), one copy for the batch     (P = 0: may be NULL)
@@ -388,8 +388,8 @@ int sid_shared_attn_fwd(const void* q, const long long* q_stride, const sid_kv_s
 
 /*
  * Group normalisation with an activation, channels last.
- * Stands for GroupNorm32 + SiLU of the host network's ResBlocks (ldm/modules/diffusionmodules/openaimodel.py:219-263) and
- * the GroupNorm of SpatialTransformer (ldm/modules/attention.py:695-717), on tensors with the channels contiguous.
+ * Stands for GroupNorm32 + SiLU of the host network's ResBlocks (ldm/modules/diffusionmodules/openaimodel.py) and
+ * the GroupNorm of SpatialTransformer (ldm/modules/attention.py), on tensors with the channels contiguous.
  *   x, y, dy, dx  (B, N, C), C contiguous (an NCHW tensor in channels-last memory has N = H*W)
  *   weight, bias  (C) f32, either may be NULL (ones / zeros)
  *   mean, rstd    (B, G) f32: written by the forward, read by the backward

@@ -239,7 +239,7 @@ class CrossAttention(nn.Module):
 
     def _shared(self, q, kv, logit_scale, q_layout, b, compute):
         """Single-block attention on one 8-bit copy of a style's keys and values (FeatureStore.quantize), which every image of
-        the batch reads: the reference repeats the pair b times (:577-578).  compute 'f16' / 'bf16' is the type of the queries,
+        the batch reads: the reference repeats the pair b times.  compute 'f16' / 'bf16' is the type of the queries,
         probabilities and read-back values; 'fp32', and temperatures the shared kernel does not take, run the plain kernel on
         the pair read back as numbers."""
         h, d = self.heads, q.shape[-1] // (self.heads if q_layout == "bnhd" else 1)

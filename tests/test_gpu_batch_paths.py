@@ -309,3 +309,55 @@ def test_scratch_is_the_calls_own():
         for i in range(2):
             for a, b, c in zip(outs[i], want[i], eager[i]):
                 assert torch.equal(a, b) and torch.equal(c, b)
+
+
+def test_threads_on_one_stream():
+    """Calls of two threads on one stream interleave their launches; every call's partial results are its own."""
+    import threading
+    torch.manual_seed(9)
+    q = [torch.randn(2, 8, 1, 64, device=DEV, dtype=torch.float16) for _ in range(2)]
+    pre = [tuple(torch.randn(8, 4096, 64, device=DEV, dtype=torch.float16) for _ in range(2)) for _ in range(2)]
+    x = [torch.randn(2, 70, 64, 64, device=DEV).permute(0, 3, 1, 2) for _ in range(2)]
+    call = lambda i: (ops.shared_prefix_attention(q[i], pre[i]), ops.group_norm_act(x[i], 1))
+    want, bad = [call(i) for i in range(2)], []
+
+    def work(i):
+        for _ in range(100):
+            if not all(torch.equal(a, b) for a, b in zip(call(i), want[i])):
+                bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_training_step_captured():
+    """Forward and backward of the group norm in one graph, replayed on new values."""
+    torch.manual_seed(10)
+    x = torch.randn(2, 30, 30, 64, device=DEV).permute(0, 3, 1, 2).requires_grad_()
+    w, b = (torch.randn(64, device=DEV).requires_grad_() for _ in range(2))
+    dy = torch.randn(2, 30, 30, 64, device=DEV).permute(0, 3, 1, 2)
+
+    def step():
+        y = ops.group_norm_act(x, 4, w, b)
+        return (y.detach(),) + torch.autograd.grad(y, (x, w, b), dy)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = step()
+    for _ in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(2, 30, 30, 64, device=DEV).permute(0, 3, 1, 2))
+        graph.replay()
+        got = [t.clone() for t in out]
+        for a, c in zip(got, step()):
+            assert torch.equal(a, c)
+        torch.cuda.synchronize()
