@@ -830,9 +830,10 @@ Plan make_plan(int B, int N, int C, int G, int dtype, uintptr_t addr, bool bwd) 
     const int vb = vec_bytes((long long)Cg * es, addr, es), cv = Cg * es / vb;
     // Slices above 64 KB go by passes where the resident kernel's few workgroups would read them alone (forward, bf16: 64 x 64 x
     // 320 of one image 20.5 us resident, 17.2 in passes; of four, 18.7 and 26.9) and always backward, where a thread holds two
-    // tensors (64 x 64 x 320 of sixteen images: 74 us resident, 60 in passes; of one, 36 and 24).
+    // tensors (64 x 64 x 320 of sixteen images: 74 us resident, 60 in passes; of one, 36 and 24), and with an odd number of 16-bit
+    // channels a group, whose pieces only go two bytes at a time (64 x 64 x 480 of sixteen images: 69 and 45).
     const bool large = (size_t)N * Cg * es > (64u << 10);
-    if (cv <= 1024 && !(large && (bwd || (long long)B * G <= 64))) {
+    if (cv <= 1024 && !(large && (bwd || vb == 2 || (long long)B * G <= 64))) {
         for (int threads = 256; threads <= 1024 && !pl.nv; threads *= 2) {
             if (cv > threads) continue;
             const int rows = (N + threads / cv - 1) / (threads / cv);
@@ -846,10 +847,11 @@ Plan make_plan(int B, int N, int C, int G, int dtype, uintptr_t addr, bool bwd) 
     pl.vb = vb;
     pl.gc = 1;
     if (!bwd && pl.nv) {
-        // Neighbouring groups in one workgroup while a row's piece is below a cache line, the slice still fits and there are
-        // workgroups for every CU: a piece costs an L2 request whatever its length (16 x 64 x 64 x 320, 20-byte pieces:
-        // 34.5 us with one group a workgroup, 32 with two).
-        for (int gc = 2; gc <= kCluster && G % gc == 0 && (long long)B * G / gc >= 256 && gc * cv <= 1024 && gc * Cg * es <= 128; gc *= 2) {
+        // Neighbouring groups in one workgroup while a row's piece is below a cache line, the slice still fits, there are
+        // workgroups for every CU and enough rows: a piece costs an L2 request whatever its length, a workgroup of several
+        // groups has twice the threads to bring together (16 images of 320 channels, one group and two: 64 x 64 34.2 and 31.8 us,
+        // 48 x 48 20.7 both, 32 x 32 11.5 and 14.9, 16 x 16 5.6 and 9.4).
+        for (int gc = 2; gc <= kCluster && G % gc == 0 && N >= 2560 && (long long)B * G / gc >= 256 && gc * cv <= 1024 && gc * Cg * es <= 128; gc *= 2) {
             const int rows = (N + 1024 / (gc * cv) - 1) / (1024 / (gc * cv));
             for (int i = 0; i < 3; ++i)
                 if (rows <= vectors_in(kFwdRegs[i], vb)) { pl.gc = gc; pl.threads = 1024; pl.nv = vectors_in(kFwdRegs[i], vb); break; }
