@@ -12,7 +12,7 @@ LIB = os.path.join(HERE, "libsid.so")
 SOURCES = ["sid_common.cpp", "sid_attn.hip", "sid_attn_bf16.hip", "sid_attn_x3.hip", "sid_attn_f16.hip", "sid_attn_wide.hip", "sid_attn_small.hip", "sid_mask.hip", "sid_hf.hip", "sid_adain.hip",
            "sid_kv.hip", "sid_norm.hip", "sid_shared.hip", "sid_shared_bf16.hip", "sid_shared_f16.hip",
            "sid_shared_bf16_codes.hip", "sid_shared_f16_codes.hip"]
-COMMON = [os.path.join(CSRC, "sid_common.h"), os.path.join(ROOT, "include", "sid.h")]
+COMMON = [os.path.join(CSRC, "sid_common.h"), os.path.join(ROOT, "include", "sid.h"), os.path.abspath(__file__)]
 KERNEL_HEADERS = {"sid_attn": "sid_attn_kernel.hpp", "sid_shared": "sid_shared_kernel.hpp"}     # by source prefix
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -amdgpu-mfma-vgpr-form: MFMA accumulators stay in the VGPRs the VALU softmax reads and rescales;
