@@ -894,7 +894,8 @@ int check_shape(int B, int N, int C, int G, int dtype) {
     SID_CHECK_ARG(B >= 1 && N >= 1 && C >= 1 && G >= 1, "B, N, C, G must be >= 1");
     SID_CHECK_ARG(C % G == 0, "%d channels do not divide into %d groups", C, G);
     SID_CHECK_ARG(dtype == SID_DTYPE_F32 || dtype == SID_DTYPE_BF16 || dtype == SID_DTYPE_F16, "unknown dtype %d", dtype);
-    SID_CHECK_ARG((long long)B * N * C < (1LL << 40) && (long long)N * (C / G) < (1LL << 31) && (long long)B * C < (1LL << 31) &&
+    // rows are 32-bit integers, and the passes count up to 8 rows of 512 threads and a chunk's rounding (2048 rows at most) past N
+    SID_CHECK_ARG((long long)B * N * C < (1LL << 40) && (long long)N * (C / G) < (1LL << 31) - (1 << 16) && (long long)B * C < (1LL << 31) &&
                   (long long)B * G < (1 << 30) && B < 65536, "tensor too large");
     return SID_OK;
 }

@@ -1,0 +1,31 @@
+"""The largest sizes that the 8-bit cache, shared-prefix attention and group norm take: what their index arithmetic or a launch
+cannot hold is refused on the host, before any GPU call."""
+import pytest
+
+from style_transfer_amd import lib
+
+A = 1 << 20                 # an aligned address that nothing reads
+
+
+def norm(B, N, C, G, dtype=lib.DTYPE_BF16, backward=False, ws_bytes=0):
+    """No workspace: what passes the size checks and takes the passes ends with -12, before a launch."""
+    L = lib.load()
+    if backward:
+        rc = L.sid_group_norm_act_bwd(A, A, A, A, A, A, A, A, A, B, N, C, G, 1, dtype, A, ws_bytes, None)
+    else:
+        rc = L.sid_group_norm_act_fwd(A, A, A, A, A, A, B, N, C, G, 1e-5, 1, dtype, A, ws_bytes, None)
+    return rc, L.sid_last_error().decode()
+
+
+@pytest.mark.parametrize("N", [2 ** 31 - 1, 2 ** 31 - 4096, 2 ** 31 - 2 ** 16])
+def test_group_norm_rows_near_31_bits(N):
+    """A pass walks rows in 32-bit integers, up to eight rows of 512 threads and one chunk's rounding ahead of the last row:
+    within 2^16 of 2^31 the row behind the end would be negative, and read."""
+    L = lib.load()
+    assert L.sid_group_norm_workspace_bytes(1, N, 1, 1, lib.DTYPE_BF16, 0) == 0 and "too large" in L.sid_last_error().decode()
+    for backward in (False, True):
+        rc, msg = norm(1, N, 1, 1, backward=backward)
+        assert rc == -22 and "too large" in msg
+    # the largest that is taken: refused here for its workspace alone
+    assert L.sid_group_norm_workspace_bytes(1, 2 ** 31 - 2 ** 16 - 1, 1, 1, lib.DTYPE_BF16, 0) > 256
+    assert norm(1, 2 ** 31 - 2 ** 16 - 1, 1, 1)[0] == norm(1, 2 ** 31 - 2 ** 16 - 1, 1, 1, backward=True)[0] == -12
