@@ -609,7 +609,31 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
         own_len: int32 (B,) tensor on the device, how many of its own keys each sequence has (clamped to [0, S]).
         causal: query i of a sequence sees its own keys j <= own_len - n + i.
     Hq must be a multiple of Hkv (query head h reads key/value head h // (Hq // Hkv)).  scale: d ** -0.5 if None.
-    -> (B, n, Hq*d) of q's dtype.  A query that sees no key gives zeros.  Forward only, like the attention calls above."""
+    -> (B, n, Hq*d) of q's dtype.  A query that sees no key gives zeros.  Forward only: where q or a 16-bit key or value
+    requires a gradient, a backward pass through the result raises an error, and `out` is refused."""
+    if torch.is_grad_enabled():
+        pairs = [p for p in (prefix, own) if p is not None and not isinstance(p, QuantKV)]
+        tracked = [t for t in (q, *(t for p in pairs for t in p)) if t.requires_grad]
+        if tracked:
+            if out is not None:
+                raise RuntimeError("shared_prefix_attention: out= takes no inputs that require a gradient")
+            return _SharedPrefixForward.apply(lambda: _shared_prefix(q, prefix, own, own_len, causal, scale, prefix_len, None), *tracked)
+    return _shared_prefix(q, prefix, own, own_len, causal, scale, prefix_len, out)
+
+
+class _SharedPrefixForward(torch.autograd.Function):
+    """The call's place in an autograd graph: without it the result would be cut off from q, keys and values silently."""
+
+    @staticmethod
+    def forward(ctx, call, *tracked):
+        return call()
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise RuntimeError("shared_prefix_attention is forward only: it has no gradient for q, keys and values")
+
+
+def _shared_prefix(q, prefix, own, own_len, causal, scale, prefix_len, out):
     L = _lib.load()
     dev = q.device
     if q.dim() != 4:
