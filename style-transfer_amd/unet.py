@@ -68,6 +68,12 @@ class GroupNorm32(nn.GroupNorm):
         return super().forward(x.float()).type(x.dtype)
 
 
+def unwatched(*modules):
+    """Whether `modules` may be passed over: no hook of theirs (or of all modules) waits for their call."""
+    return not (torch.nn.modules.module._has_any_global_hook()
+                or any(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks for m in modules))
+
+
 def norm_act(norm, x, act):
     """A GroupNorm module and the activation behind it in one kernel, channels last."""
     return ops.group_norm_act(x.contiguous(memory_format=torch.channels_last), norm.num_groups, norm.weight, norm.bias,
@@ -93,13 +99,16 @@ class ResBlock(nn.Module):
     def forward(self, x, emb, out_layers_injected=None):
         return self._forward(x, emb, out_layers_injected)
 
+    def _fused(self, layers):
+        return self.fused_norm and unwatched(layers, layers[0], layers[1])
+
     def _forward(self, x, emb, out_layers_injected=None):
-        h = self.in_layers[2](norm_act(self.in_layers[0], x, "silu")) if self.fused_norm else self.in_layers(x)
+        h = self.in_layers[2](norm_act(self.in_layers[0], x, "silu")) if self._fused(self.in_layers) else self.in_layers(x)
         if out_layers_injected is not None:
             h = torch.cat([out_layers_injected] * x.shape[0])
         else:
             h = h + self.emb_layers(emb).type(h.dtype)[..., None, None]
-            h = self.out_layers[2:](norm_act(self.out_layers[0], h, "silu")) if self.fused_norm else self.out_layers(h)
+            h = self.out_layers[2:](norm_act(self.out_layers[0], h, "silu")) if self._fused(self.out_layers) else self.out_layers(h)
         self.out_skip = self.skip_connection(x)
         self.out_h = h
         return self.out_skip + h
@@ -174,7 +183,7 @@ class SpatialTransformer(nn.Module):
 
     def forward(self, x, context=None, **attn_kw):
         b, c, h, w = x.shape
-        y = norm_act(self.norm, x, "none") if self.fused_norm else self.norm(x)
+        y = norm_act(self.norm, x, "none") if self.fused_norm and unwatched(self.norm) else self.norm(x)
         y = self.proj_in(y).reshape(b, -1, h * w).transpose(1, 2)                  # b (h w) c
         for blk in self.transformer_blocks:
             y = blk(y, context=context, **attn_kw)
@@ -242,7 +251,8 @@ class UNetModel(nn.Module):
 
     def use_channels_last(self):
         """Weights and activations in channels-last memory, every group norm and the SiLU behind it as one kernel
-        (ops.group_norm_act).  Parameter names and the results' meaning stay; the sums round in another order."""
+        (ops.group_norm_act).  Parameter names and the results' meaning stay; the sums round in another order.  Where a
+        norm, its SiLU or the Sequential around them carries a hook, these modules run by themselves, and the hook with them."""
         self.to(memory_format=torch.channels_last)
         for m in self.modules():
             if isinstance(m, (ResBlock, SpatialTransformer, UNetModel)):
@@ -267,6 +277,6 @@ class UNetModel(nn.Module):
         for i, blk in enumerate(self.output_blocks):
             kw, out_layers = route_injected(injected_features, i)
             h = blk(torch.cat([h, hs.pop()], dim=1), emb, context, out_layers_injected=out_layers, **kw)
-        if self.fused_norm:
+        if self.fused_norm and unwatched(self.out, self.out[0], self.out[1]):
             return self.out[2](norm_act(self.out[0], h, "silu")).contiguous()
-        return self.out(h)
+        return self.out(h).contiguous() if self.fused_norm else self.out(h)
