@@ -394,7 +394,8 @@ int sid_shared_attn_fwd(const void* q, const long long* q_stride, const sid_kv_s
  *   weight, bias  (C) f32, either may be NULL (ones / zeros)
  *   mean, rstd    (B, G) f32: written by the forward, read by the backward
  *   y = act((x - mean) * rstd * weight + bias), biased variance, statistics in f32
- *   dweight, dbias  (C) f32 sums over the batch, either may be NULL.  Results repeat bit for bit (no atomics).
+ *   dx, dweight, dbias  each may be NULL, not all three: that gradient is not computed.  dweight and dbias are (C) f32
+ *                       sums over the batch.  Results repeat bit for bit (no atomics).
  */
 size_t sid_group_norm_workspace_bytes(int B, int N, int C, int G, int dtype, int backward);
 

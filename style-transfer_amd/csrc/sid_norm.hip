@@ -152,7 +152,7 @@ __device__ __forceinline__ void join(float& n, float& mean, float& m2, float nb,
 
 struct NormParams {
     const char *x, *dy;
-    char* out;                    // y (forward) or dx (backward)
+    char* out;                    // y (forward) or dx (backward, or null)
     const float *w, *b;           // (C) or null: ones / zeros
     float *mean, *rstd;           // (B, G): written by the forward, read by the backward
     float2* part;                 // passes: [B][chunk][C]; resident backward: [B][C]
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(1024) gn_bwd_resident(NormParams p) {
     block_sum<2>(s, sm);                            // its barriers also order the channel sums above
     const float inv_n = 1.f / ((float)p.N * (float)p.Cg);
     const float s1 = s[0] * inv_n, s2 = s[1] * inv_n;
-    if (live)
+    if (live && p.out)
 #pragma unroll
         for (int k = 0; k < NV; ++k)
             if (row0 + k * rp < p.N) {
@@ -1017,7 +1017,8 @@ extern "C" int sid_group_norm_act_bwd(const void* dy, const void* x, const float
                                       const float* mean, const float* rstd, void* dx, float* dweight, float* dbias,
                                       int B, int N, int C, int G, int act, int dtype,
                                       void* workspace, size_t workspace_bytes, void* stream) {
-    SID_CHECK_ARG(dy && x && mean && rstd && dx, "NULL tensor pointer");
+    SID_CHECK_ARG(dy && x && mean && rstd, "NULL tensor pointer");
+    SID_CHECK_ARG(dx || dweight || dbias, "no gradient asked for");
     if (int rc = check_shape(B, N, C, G, dtype)) return rc;
     SID_CHECK_ARG(act == SID_ACT_NONE || act == SID_ACT_SILU, "unknown activation %d", act);
     SID_CHECK_ARG(aligned_to_elements((uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx, dtype), "tensors must be aligned to their elements");

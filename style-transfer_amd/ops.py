@@ -769,8 +769,8 @@ def _norm_backward(ctx, dy):
     dev = x.device
     if dy.dtype != x.dtype or dy.stride() != x.stride():
         dy = dy.to(x.dtype).contiguous(memory_format=torch.channels_last if x.dim() == 4 else torch.contiguous_format)
-    _, need_w, need_b = ctx.needs_input_grad[:3]
-    dx = torch.empty_like(x)
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    dx = torch.empty_like(x) if need_x else None
     dw = torch.empty_like(weight) if need_w else None
     db = torch.empty_like(bias) if need_b else None
     need = _scratch_bytes("sid_group_norm_workspace_bytes", B, N, C, G, dt, 1)
@@ -779,7 +779,7 @@ def _norm_backward(ctx, dy):
     with _on(dev):
         _lib.check(_lib.load().sid_group_norm_act_bwd(
             dy.data_ptr(), x.data_ptr(), None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
-            sp, sp + 4 * B * G, dx.data_ptr(), dw.data_ptr() if need_w else None, db.data_ptr() if need_b else None,
+            sp, sp + 4 * B * G, dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None, db.data_ptr() if need_b else None,
             B, N, C, G, act, dt, ws.data_ptr(), need, _stream(dev)))
     return dx, dw, db, None, None, None
 

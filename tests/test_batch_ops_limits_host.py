@@ -29,3 +29,11 @@ def test_group_norm_rows_near_31_bits(N):
     # the largest that is taken: refused here for its workspace alone
     assert L.sid_group_norm_workspace_bytes(1, 2 ** 31 - 2 ** 16 - 1, 1, 1, lib.DTYPE_BF16, 0) > 256
     assert norm(1, 2 ** 31 - 2 ** 16 - 1, 1, 1)[0] == norm(1, 2 ** 31 - 2 ** 16 - 1, 1, 1, backward=True)[0] == -12
+
+
+def test_group_norm_backward_takes_any_gradient_alone():
+    """No dx: refused for its workspace alone here, as with it.  None of the three: nothing to do."""
+    L = lib.load()
+    call = lambda dx, dw, db: L.sid_group_norm_act_bwd(A, A, A, A, A, A, dx, dw, db, 1, 1 << 16, 64, 8, 1, lib.DTYPE_F32, A, 0, None)
+    assert call(A, A, A) == call(None, A, A) == call(None, None, A) == call(None, A, None) == call(A, None, None) == -12
+    assert call(None, None, None) == -22 and "no gradient" in L.sid_last_error().decode()
