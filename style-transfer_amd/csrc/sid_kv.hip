@@ -230,7 +230,7 @@ extern "C" int sid_kv_cache_write(const void* k, const void* v, const long long*
     p.H = H; p.n = n; p.S = S; p.d = d;
     while ((8 << p.lanes_log2) < d) ++p.lanes_log2;
     const long long per_block = 256 >> p.lanes_log2, grid = (p.rows + per_block - 1) / per_block;
-    SID_CHECK_ARG(grid < (1LL << 31), "too many rows");
+    SID_CHECK_ARG(grid < (1LL << 24), "too many rows");            // a launch holds fewer than 2^32 threads in x
     if (dtype == SID_DTYPE_F32) return launch_write<SID_DTYPE_F32>(p, fmt, (unsigned)grid, (hipStream_t)stream);
     if (dtype == SID_DTYPE_BF16) return launch_write<SID_DTYPE_BF16>(p, fmt, (unsigned)grid, (hipStream_t)stream);
     return launch_write<SID_DTYPE_F16>(p, fmt, (unsigned)grid, (hipStream_t)stream);

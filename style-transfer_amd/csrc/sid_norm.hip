@@ -890,6 +890,15 @@ Plan make_plan(int B, int N, int C, int G, int dtype, uintptr_t addr, bool bwd) 
 
 size_t plan_bytes(const Plan& pl) { return pl.part_bytes + pl.sums_bytes + pl.chan_bytes; }
 
+// A launch holds fewer than 2^32 threads in x and 2^16 workgroups in z.
+int check_launch(const Plan& pl, int B, int C, int G, int dtype) {
+    const long long items = (long long)B * (G / pl.gc) + kXcd;                    // resident workgroups, or those of a join
+    const long long slabs = ((long long)C * (dtype == SID_DTYPE_F32 ? 4 : 2) / pl.vb + 511) / 512;
+    const bool fits = pl.nv ? items * pl.threads < (1LL << 32) : slabs < (1 << 16) && (pl.fold || items * 256 < (1LL << 32));
+    SID_CHECK_ARG(fits && C <= (1 << 27) - 32, "tensor too large: %d channels, %lld groups", C, (long long)B * G);      // 32 threads a channel
+    return SID_OK;
+}
+
 int check_shape(int B, int N, int C, int G, int dtype) {
     SID_CHECK_ARG(B >= 1 && N >= 1 && C >= 1 && G >= 1, "B, N, C, G must be >= 1");
     SID_CHECK_ARG(C % G == 0, "%d channels do not divide into %d groups", C, G);
@@ -1002,6 +1011,7 @@ extern "C" int sid_group_norm_act_fwd(const void* x, const float* weight, const 
     SID_CHECK_ARG(aligned_to_elements((uintptr_t)x | (uintptr_t)y, dtype), "tensors must be aligned to their elements");
     SID_CHECK_ARG(eps >= 0.f, "eps must not be negative");
     const Plan pl = make_plan(B, N, C, G, dtype, (uintptr_t)x | (uintptr_t)y, false);
+    if (int rc = check_launch(pl, B, C, G, dtype)) return rc;
     if (plan_bytes(pl) > workspace_bytes) return sid::fail(SID_ENOMEM, "workspace of %zu bytes, %zu needed", workspace_bytes, plan_bytes(pl));
     SID_CHECK_ARG(plan_bytes(pl) == 0 || (workspace && (uintptr_t)workspace % 256 == 0), "workspace must be 256-byte aligned");
     NormParams p = params_of(B, N, C, G, act);
@@ -1023,6 +1033,7 @@ extern "C" int sid_group_norm_act_bwd(const void* dy, const void* x, const float
     SID_CHECK_ARG(act == SID_ACT_NONE || act == SID_ACT_SILU, "unknown activation %d", act);
     SID_CHECK_ARG(aligned_to_elements((uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx, dtype), "tensors must be aligned to their elements");
     const Plan pl = make_plan(B, N, C, G, dtype, (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx, true);
+    if (int rc = check_launch(pl, B, C, G, dtype)) return rc;
     if (plan_bytes(pl) > workspace_bytes) return sid::fail(SID_ENOMEM, "workspace of %zu bytes, %zu needed", workspace_bytes, plan_bytes(pl));
     SID_CHECK_ARG(workspace && (uintptr_t)workspace % 256 == 0, "workspace must be 256-byte aligned");
     NormParams p = params_of(B, N, C, G, act);

@@ -177,6 +177,9 @@ extern "C" int sid_shared_attn_fwd(const void* q, const long long* q_stride, con
 
     const int fmt[2] = {P ? prefix->fmt : SID_KV_NONE, S ? own->fmt : SID_KV_NONE};
     const Plan pl = make_plan(B, Hkv, Hq / Hkv, n, d, P, S, P && S && fmt[0] != fmt[1]);
+    long long workgroups = 0;
+    for (int g = 0; g < pl.groups; ++g) workgroups += padded(pl.g[g].items);
+    SID_CHECK_ARG(workgroups < (1 << 24), "too many rows");                       // a launch holds fewer than 2^32 threads in x
     const long long rows = (long long)B * n * Hq;
     const size_t need = plan_bytes(pl, rows, d);
     if (need > workspace_bytes) return sid::fail(SID_ENOMEM, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
