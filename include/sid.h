@@ -399,6 +399,14 @@ int sid_shared_attn_fwd(const void* q, const long long* q_stride, const sid_kv_s
  */
 size_t sid_group_norm_workspace_bytes(int B, int N, int C, int G, int dtype, int backward);
 
+/*
+ * The form a call takes for tensors on 16-byte boundaries (host only; for tests and for callers that look into a time):
+ *   plan[0] vectors of the slice that a thread holds (0: by passes)   plan[1] bytes of a vector
+ *   plan[2] threads of a workgroup                                    plan[3] groups of a workgroup
+ *   plan[4] row chunks of an image (by passes)                        plan[5] 1: the output pass joins the chunks itself
+ */
+int sid_group_norm_plan(int B, int N, int C, int G, int dtype, int backward, int plan[6]);
+
 int sid_group_norm_act_fwd(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd,
                            int B, int N, int C, int G, float eps, int act, int dtype,
                            void* workspace, size_t workspace_bytes, void* stream);

@@ -1002,6 +1002,14 @@ extern "C" size_t sid_group_norm_workspace_bytes(int B, int N, int C, int G, int
     return most;
 }
 
+extern "C" int sid_group_norm_plan(int B, int N, int C, int G, int dtype, int backward, int plan[6]) {
+    SID_CHECK_ARG(plan, "NULL pointer");
+    if (int rc = check_shape(B, N, C, G, dtype)) return rc;
+    const Plan pl = make_plan(B, N, C, G, dtype, 0, backward != 0);
+    plan[0] = pl.nv; plan[1] = pl.vb; plan[2] = pl.nv ? pl.threads : 512; plan[3] = pl.gc; plan[4] = pl.chunks; plan[5] = pl.fold;
+    return SID_OK;
+}
+
 extern "C" int sid_group_norm_act_fwd(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd,
                                       int B, int N, int C, int G, float eps, int act, int dtype,
                                       void* workspace, size_t workspace_bytes, void* stream) {

@@ -58,6 +58,7 @@ SIGNATURES = {
     "sid_shared_attn_workspace_bytes": (_sz, [_i] * 8),
     "sid_shared_attn_fwd": (_i, [_vp] * 6 + [_i] * 7 + [_f] + [_i] * 2 + [_vp, _sz, _vp]),
     "sid_group_norm_workspace_bytes": (_sz, [_i] * 6),
+    "sid_group_norm_plan": (_i, [_i] * 6 + [_c.POINTER(_c.c_int)]),
     "sid_group_norm_act_fwd": (_i, [_vp] * 6 + [_i] * 4 + [_f] + [_i] * 2 + [_vp, _sz, _vp]),
     "sid_group_norm_act_bwd": (_i, [_vp] * 9 + [_i] * 6 + [_vp, _sz, _vp]),
 }
