@@ -612,13 +612,22 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
     -> (B, n, Hq*d) of q's dtype.  A query that sees no key gives zeros.  Forward only: where q or a 16-bit key or value
     requires a gradient, a backward pass through the result raises an error, and `out` is refused."""
     if torch.is_grad_enabled():
-        pairs = [p for p in (prefix, own) if p is not None and not isinstance(p, QuantKV)]
-        tracked = [t for t in (q, *(t for p in pairs for t in p)) if t.requires_grad]
-        if tracked:
+        tracked, prefix = _tracked(prefix)
+        tracked_own, own = _tracked(own)
+        if tracked or tracked_own or q.requires_grad:
             if out is not None:
                 raise RuntimeError("shared_prefix_attention: out= takes no inputs that require a gradient")
-            return _SharedPrefixForward.apply(lambda: _shared_prefix(q, prefix, own, own_len, causal, scale, prefix_len, None), *tracked)
+            inputs = [t for p in ((q,), prefix, own) if p is not None and not isinstance(p, QuantKV) for t in p]
+            return _SharedPrefixForward.apply(lambda: _shared_prefix(q, prefix, own, own_len, causal, scale, prefix_len, None), *inputs)
     return _shared_prefix(q, prefix, own, own_len, causal, scale, prefix_len, out)
+
+
+def _tracked(part):
+    """Whether a key or value of the part requires a gradient; the part, its pair as a tuple."""
+    if part is None or isinstance(part, QuantKV):
+        return False, part
+    k, v = part = tuple(part)
+    return k.requires_grad or v.requires_grad, part
 
 
 class _SharedPrefixForward(torch.autograd.Function):

@@ -60,3 +60,16 @@ def test_attention_module_on_codes():
     frozen.to_q.requires_grad_(False)
     call(frozen).sum().backward()
     assert torch.isfinite(frozen.to_out[0].weight.grad).all() and float(frozen.to_out[0].weight.grad.abs().sum()) > 0
+
+
+def test_pairs_of_any_kind():
+    """A pair may be a tuple, a list, a stacked tensor or an iterator, with gradients tracked or not."""
+    o = ops()
+    q, pre, own = tensors()
+    want = o.shared_prefix_attention(q, pre, own)
+    for make in (list, torch.stack, iter):
+        assert torch.equal(o.shared_prefix_attention(q, make(pre), make(own)), want)
+        with torch.no_grad():
+            assert torch.equal(o.shared_prefix_attention(q, make(pre), make(own)), want)
+    pre[1].requires_grad_()
+    assert o.shared_prefix_attention(q, iter(pre), own).requires_grad
