@@ -343,6 +343,8 @@ int sid_masked_adain(const void* cnt, const void* sty_char, const void* sty_back
  *   k_strides, v_strides  HOST arrays of three: elements from sequence to sequence, head to head, token to token (the
  *                         last dimension is contiguous); rows 16-byte aligned.
  *   start                 (B) int32 on the device;  length: (B) int32 on the device, or NULL: n for all.
+ *   B * H < 2^16; a write of fewer than 2^24 workgroups (of 256 / (d / 8, rounded up to a power of two) rows); a read of
+ *   n * (d / 8)^2 < 2^32 about.
  */
 int sid_kv_cache_write(const void* k, const void* v, const long long* k_strides, const long long* v_strides,
                        void* k_codes, void* v_codes, float* k_scale, float* v_scale,
@@ -369,7 +371,8 @@ int sid_kv_cache_read(const void* k_codes, const void* v_codes, const float* k_s
  * whatever they hold.  Products run at 16-bit operands (8-bit codes become numbers of `dtype` first), probabilities are
  * rounded to `dtype` for the second product.  A query that sees a non-finite value within 64 keys of the causal edge
  * comes out NaN in all its columns (elsewhere: in the columns of that value).
- * scale: positive and finite.
+ * scale: positive and finite.  A value that is code * scale and exceeds the type's range is infinite.  Forward only.
+ * B * n * Hq < 2^24, P and S < 2^30.
  */
 typedef struct sid_kv_source {
     const void *k, *v;                 /* 16-bit numbers (fmt SID_KV_NONE) or codes */
@@ -396,6 +399,7 @@ int sid_shared_attn_fwd(const void* q, const long long* q_stride, const sid_kv_s
  *   y = act((x - mean) * rstd * weight + bias), biased variance, statistics in f32
  *   dx, dweight, dbias  each may be NULL, not all three: that gradient is not computed.  dweight and dbias are (C) f32
  *                       sums over the batch.  Results repeat bit for bit (no atomics).
+ *   B < 2^16, N * (C / G) < 2^31 - 2^16, C <= 2^27 - 32, B * N * C < 2^40.
  */
 size_t sid_group_norm_workspace_bytes(int B, int N, int C, int G, int dtype, int backward);
 

@@ -16,9 +16,11 @@
 //             do not fit and for batches with too few slices to fill the chip.
 // Sums, statistics and gradients of w and b are f32; variances are combined from (count, mean, centred sum) triples,
 // so a large mean costs no digits.  No atomics: sums have one order, results repeat bit for bit.
-// Measured (bf16): forward 8 x 64 x 64 x 960 resident 32 us, 3.9 TB/s; 16 x 64 x 64 x 320 32 us, 2.6 TB/s (40-byte row
-// pieces); 8 x 8 x 1280 f32 4.2 us.  Backward 8 x 64 x 64 x 960 by passes 84 us: sums 31 us at 4.1 TB/s, output 41 us at
-// 4.7 TB/s, gradients of w and b 4 us; 2 x 16 x 16 x 640 resident 7.6 us + 2.8 us (one image: no second launch).
+// Measured (bf16): forward 8 x 64 x 64 x 960 resident 34 us on an input that the 256 MB cache holds, 45 us (2.8 TB/s) on one
+// that comes from memory; 16 x 64 x 64 x 320 33 us, 2.5 TB/s (4-byte loads: a vector divides ONE group's 20 bytes, also where
+// a workgroup holds two); 8 x 8 x 1280 f32 4.8 us; one image of 64 x 64 x 320 by passes 17 us bf16, 13 us f32.
+// Backward 8 x 64 x 64 x 960 by passes 80 us: sums 32 us at 3.9 TB/s, output 43 us at 4.4 TB/s, gradients of w and b 5 us;
+// 2 x 16 x 16 x 640 resident 7.7 us + 2.5 us behind a forward of 5.2 us (one image: no second launch).
 #include "sid_common.h"
 
 #include <cstdint>

@@ -214,7 +214,8 @@ extern "C" int sid_shared_attn_fwd(const void* q, const long long* q_stride, con
         g += both ? 2 : 1;
     }
     if (need) {
-        // quads of a row to a power of two; slots shared by up to eight threads while that leaves each one a few
+        // quads of a row to a power of two; slots shared by up to 16 threads (d <= 64; 8 to 128, 4 above) while that leaves
+        // each one a few
         int log_q = 4, log_sg = 0;
         while ((4 << log_q) < d) ++log_q;
         while (log_sg < 8 - log_q && (4 << log_sg) < pl.slots) ++log_sg;

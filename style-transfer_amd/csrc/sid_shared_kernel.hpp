@@ -28,10 +28,14 @@
 // exactly; their scale multiplies the f32 logits, because a rounding of the keys would shift a logit by 2^-9 of the sum of
 // |q k|, twice the error of everything else at |logit| = 5), value codes times their scale, rounded once.
 //
-// Measured: 4 images of 4096 queries, 8 heads of 40, 4096 + 4096 keys 224 us, 765 TFLOP/s (bound by the exponentials and
-// conversions beside the products; d = 128 550 us, 1000 TFLOP/s); one token of 32 sequences, 32 / 8 heads of 128, 32768 + 1024 keys 50 us + 6 us to join,
-// 4.2 TB/s (bound by memory); five tokens of 16 sequences on int8 codes, 16 / 4 heads of 128, 8191 + 333 keys 27 us + 5 us,
-// one token of 4 sequences on 1023 + 128 keys 8.8 us (both bound by one workgroup's chain of loads, products and join).
+// Measured: 4 images of 4096 queries, 8 heads of 40, 4096 + 4096 keys 233 us, 740 TFLOP/s (a tile of 64 keys takes a SIMD
+// about 1930 cycles, which is its products' 900 and its vector work's 1050 one after the other; d = 128 565 us, 970 TFLOP/s);
+// one token of 32 sequences, 32 / 8 heads of 128, 32768 + 1024 keys 49 us + 6 us to join, 4.2 TB/s (bound by memory; on
+// int8 codes 49 us for both); five tokens of 16 sequences on int8 codes, 16 / 4 heads of 128, 8191 + 333 keys 28 us + 5 us
+// (21 MB of partial results written and read, and every code converted for three row tiles); one token of 4 sequences on
+// 1023 + 128 keys 6.4 us + 3.4 us (a workgroup's chain of loads, products and join).  Heads of 160 and 256, 4 images of 2048
+// queries on 2048 + 2048 keys: 440 and 629 us, 390 and 437 TFLOP/s (Rows16 reads each K fragment right before its product,
+// for 16 rows only).
 #pragma once
 #include "sid_common.h"
 

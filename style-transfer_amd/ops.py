@@ -540,7 +540,8 @@ def kv_cache_write(cache, k, v, start=0, length=None):
     """Quantise k, v (B, H, n, d) (float32, bfloat16 or float16; any strides with d contiguous) into positions start[b] + i of
     sequence b.  start: an int, or an int32 (B,) tensor on the device (nothing is read back, so a decoding step can be
     captured in a HIP graph).  length: int32 (B,) tensor, rows i >= length[b] are padding and not written; None: all n.
-    Positions outside the cache are skipped; everything else in it stays as it was.  One launch."""
+    Positions outside the cache are skipped; everything else in it stays as it was.  One launch, and a second that fills a
+    tensor with an int start."""
     L = _lib.load()
     dev = cache.device
     if k.shape != v.shape or k.dtype != v.dtype or k.dim() != 4:
@@ -566,7 +567,7 @@ def kv_cache_write(cache, k, v, start=0, length=None):
 
 def kv_cache_read(cache, start, n, dtype=torch.bfloat16):
     """The n positions from start[b] on (int, or int32 (B,) tensor on the device) as numbers: k, v (B, H, n, d) in `dtype`.
-    Positions outside the cache give zeros.  One launch."""
+    Positions outside the cache give zeros.  One launch, and a second that fills a tensor with an int start."""
     L = _lib.load()
     dev = cache.device
     if dtype not in _DTYPES3:
