@@ -816,7 +816,8 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="silu"):
 
     x (B, C, H, W) in channels-last memory, or tokens (B, N, C) contiguous; float32, bfloat16 or float16.  weight, bias:
     float32 (C,) or None (other float types are cast, with gradients).  act: "silu" or "none".  Statistics, gradients of
-    weight and bias and all arithmetic are float32; y has x's dtype and memory order.  Needs at least one value."""
+    weight and bias and all arithmetic are float32; y has x's dtype and memory order.  Needs at least one value.  A training
+    step can be captured; as with torch's own operators, only while no eager graph of the same leaves is alive."""
     if act not in _ACTS:
         raise ValueError("act must be 'silu' or 'none', got %r" % (act,))
     eps = float(eps)
