@@ -556,6 +556,8 @@ def kv_cache_write(cache, k, v, start=0, length=None):
         length = _positions(length, B, dev)
         _need_device(dev, length)
     _need_device(dev, k, v, start)
+    if cache.k_codes.numel() == 0:               # no position to write to
+        return
     k, kp, ks = _rows16(k)
     v, vp, vs = _rows16(v)
     with _on(dev):
@@ -577,6 +579,8 @@ def kv_cache_read(cache, start, n, dtype=torch.bfloat16):
     start = _positions(start, cache.B, dev)
     _need_device(dev, start)
     shape = (cache.B, cache.H, n, cache.d)
+    if cache.k_codes.numel() == 0:               # every position is outside
+        return torch.zeros(shape, dtype=dtype, device=dev), torch.zeros(shape, dtype=dtype, device=dev)
     k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
     with _on(dev):
         _lib.check(L.sid_kv_cache_read(cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scale.data_ptr(),
