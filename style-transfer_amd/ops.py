@@ -608,7 +608,8 @@ def shared_prefix_attention(q, prefix=None, own=None, own_len=None, causal=False
     """Attention of a batch whose sequences share a prefix of keys and values, under one softmax with their own keys.
 
     q (B, Hq, n, d) bfloat16 or float16, any strides with d contiguous; n = 1 for a decoding step.
-    prefix: (k, v) of shape (Hkv, P, d), one copy for the whole batch, or a QuantKV with B = 1; None: no prefix.
+    prefix: (k, v) of shape (Hkv, P, d), one copy for the whole batch, or a QuantKV with B = 1; None: no prefix.  (Parts in
+        8 bits of head_dim 8 are copied to rows of 16 in every call.)
         prefix_len: only its first keys (an int); None: all.
     own: (k, v) of shape (B, Hkv, S, d), or a QuantKV with the batch's B; None: none.
         own_len: int32 (B,) tensor on the device, how many of its own keys each sequence has (clamped to [0, S]).
@@ -647,6 +648,26 @@ class _SharedPrefixForward(torch.autograd.Function):
         raise RuntimeError("shared_prefix_attention is forward only: it has no gradient for q, keys and values")
 
 
+def _pad8(t):
+    return torch.nn.functional.pad(t, (0, 8))
+
+
+def _sixteen(part):
+    """A part of head_dim 8 as one of 16, zeros behind every row."""
+    if part is None:
+        return None
+    if isinstance(part, QuantKV):
+        k, v = (_pad8(c.view(torch.uint8)).view(c.dtype) for c in (part.k_codes, part.v_codes))
+        return QuantKV(k, part.k_scale, v, part.v_scale)
+    return tuple(_pad8(t) for t in part)
+
+
+def _checked_out(out, shape, dtype, dev):
+    if out.shape != shape or out.dtype != dtype or not out.is_contiguous() or out.device != dev:
+        raise ValueError("out must be a contiguous %s %s on %s" % (tuple(shape), dtype, dev))
+    return out
+
+
 def _shared_prefix(q, prefix, own, own_len, causal, scale, prefix_len, out):
     L = _lib.load()
     dev = q.device
@@ -656,9 +677,11 @@ def _shared_prefix(q, prefix, own, own_len, causal, scale, prefix_len, out):
         raise TypeError("q must be bfloat16 or float16, got %s" % q.dtype)
     B, Hq, n, d = q.shape
     _need_device(dev)
-    if d == 8:                       # the kernel reads codes sixteen at a time: rows of eight become numbers first
-        prefix, own = (tuple(t[0] for t in kv_cache_read(prefix, 0, prefix.S, q.dtype)) if isinstance(prefix, QuantKV) and prefix.B == 1 else prefix,
-                       kv_cache_read(own, 0, own.S, q.dtype) if isinstance(own, QuantKV) else own)
+    if d == 8 and (isinstance(prefix, QuantKV) or isinstance(own, QuantKV)):
+        # the kernel reads codes sixteen at a time: eight zeros behind every row add nothing to a product
+        y = _shared_prefix(_pad8(q), _sixteen(prefix), _sixteen(own), own_len, causal, d ** -0.5 if scale is None else scale, prefix_len, None)
+        y = y.view(B, n, Hq, 16)[..., :8].reshape(B, n, Hq * 8)
+        return y if out is None else _checked_out(out, y.shape, y.dtype, dev).copy_(y)
     P = S = 0
     Hp = Ho = None
     src_p = src_o = alive = None
@@ -703,10 +726,7 @@ def _shared_prefix(q, prefix, own, own_len, causal, scale, prefix_len, out):
         own_len = _positions(own_len, B, dev)
         _need_device(dev, own_len)
     q, qp, qs = _rows16(q)
-    if out is None:
-        out = torch.empty((B, n, Hq * d), dtype=q.dtype, device=dev)
-    elif out.shape != (B, n, Hq * d) or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
-        raise ValueError("out must be a contiguous %s %s on %s" % ((B, n, Hq * d), q.dtype, dev))
+    out = torch.empty((B, n, Hq * d), dtype=q.dtype, device=dev) if out is None else _checked_out(out, (B, n, Hq * d), q.dtype, dev)
     ws = _call_scratch(dev, _scratch_bytes("sid_shared_attn_workspace_bytes", B, Hq, Hkv, n, d, P, S,
                                          int(P and S and fmt_p != fmt_o)))
     with _on(dev):
